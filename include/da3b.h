@@ -178,6 +178,90 @@ DA3B_API int da3b_attention_vt(const void* qkv, const void* vt, int ld_vt, int n
 DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int heads, void* out, int* status_dev,
                                     void* stream);
 
+/* ----------------------------------------------------------------------
+ * Linears in 8-bit floating point. No counterpart in the reference (its quantised linears
+ * are Q8_0, above); for callers that trade some of f16's precision for twice the
+ * tensor-core rate and half the operand bytes.
+ *
+ * A matrix [rows][K] (activations, or weights [N][K]) is held as e4m3 codes [rows][ld]
+ * (ld bytes, ld >= K and a multiple of 16, base 16-byte aligned) and one scale for each
+ * row and 128 columns: value = code * 2^(s - 127), s a byte. The scale bytes lie in
+ * "scale tiles" (16-byte aligned, da3b_fp8_scale_bytes(rows, K) bytes): 512 bytes for each
+ * 512 columns g and 128 rows t, in the order [g][t][32][4][4]; row 128 t + 32 c + l and
+ * columns from 128 (4 g + j) on have theirs at [g][t][l][c][j]. Bytes of rows and columns
+ * that the matrix does not have are never used. The tiles depend on the number of rows:
+ * pass the same `rows` everywhere.
+ *
+ * A quantised block has the smallest s with max|x| <= 448 * 2^(s - 127) (at least 0; 127
+ * for a block of zeros), codes round to nearest, ties to even. e4m3 has no infinity:
+ * infinities and NaN become NaN, and the scale is that of the block's finite values.
+ *
+ * Types: 0 f16, 1 bf16, 2 f32. All functions return 0 when launched, -100 for a null
+ * pointer or a bad code or count, -1 for sizes, leading dimensions or alignments that are
+ * not served, other negative values for launch errors. Calls with no rows do nothing.
+ * Nothing is allocated except the status word on a device's first call (make that one
+ * outside of a stream capture); any number of calls may run at once. Pointers belong to
+ * the current device, and outputs may not overlap inputs.
+ * ---------------------------------------------------------------------- */
+DA3B_API size_t da3b_fp8_scale_bytes(int rows, int K);
+
+/* x [rows][ldx] of type dtype -> codes q [rows][ldq] and scale tiles. Columns from K up to
+ * the next multiple of 16 are set to zero. */
+DA3B_API int da3b_quantize_fp8(const void* x, int dtype, int rows, int K, int ldx, void* q, int ldq, void* scales,
+                               void* stream);
+
+/* LayerNorm of f32 rows, (x - mean) / sqrt(var + eps) * gamma + beta (beta may be NULL;
+ * K <= 16384), quantised as above: the norm before a block's linears, without the f16
+ * round trip. */
+DA3B_API int da3b_layernorm_fp8(const float* x, int rows, int K, int ldx, const float* gamma, const float* beta,
+                                float eps, void* q, int ldq, void* scales, void* stream);
+
+/* y = act(x w^T + bias) of quantised x [M][K] and w [N][K]; bias f32 [N] or NULL, act as
+ * da3b_linear_f16, sums in f32.
+ *   da3b_linear_fp8:           y [M][ldo] of type out_dtype.
+ *   da3b_linear_fp8_q:         y quantised by the product's epilogue: codes out_q [M][ldo]
+ *                              (ldo a multiple of 16, columns from N on untouched) and
+ *                              scale tiles of an M x N matrix: the next linear's input.
+ *   da3b_linear_fp8_resid_f32: resid[m][n] += scale[n] * (y[m][n]) in f32 (no activation;
+ *                              scale f32 [N] or NULL), as da3b_linear_resid_f32. */
+DA3B_API int da3b_linear_fp8(const void* x, int M, int K, int ldx, const void* x_scales, const void* w, int N,
+                             int ldw, const void* w_scales, const float* bias, int act, void* out, int out_dtype,
+                             int ldo, void* stream);
+DA3B_API int da3b_linear_fp8_q(const void* x, int M, int K, int ldx, const void* x_scales, const void* w, int N,
+                               int ldw, const void* w_scales, const float* bias, int act, void* out_q, int ldo,
+                               void* out_scales, void* stream);
+DA3B_API int da3b_linear_fp8_resid_f32(const void* x, int M, int K, int ldx, const void* x_scales, const void* w,
+                                       int N, int ldw, const void* w_scales, const float* bias, const float* scale,
+                                       float* resid, int ldr, void* stream);
+
+/* Attention over a window of keys and the first few keys of each sequence, for streams of
+ * views (or prompts) too long for da3b_attention's all-to-all form: a query sees the keys
+ * around its own position and the first `sinks` ones (say the reference view's tokens).
+ * No counterpart in the reference.
+ *
+ * Sequence s has ql = q_lens[s] queries and kl = k_lens[s] keys (device arrays; NULL: q_len
+ * and k_len for all; values are clamped to [0, q_len] and [0, k_len]). Its queries are the
+ * last ones of its keys: query i stands at position p = kl - ql + i and sees key j if
+ *     j < kl  and  j <= p + right  and  (j >= p - left  or  j < sinks),
+ * left, right < 0: no limit on that side. right = 0 is causal; one query per sequence is
+ * the form for single tokens over a cache. out = sum_j softmax_j(scale * q.k_j) v_j with
+ * f32 statistics; a query that sees no key gets zeros, rows from ql on are left as they
+ * were. Keys that no query of the sequence sees are never used, whatever they hold (NaN
+ * and infinities included); a key that some query sees has to be finite for all of them.
+ *
+ * q, out [nseq][q_len][heads][head_dim], k, v [nseq][k_len][kv_heads][head_dim], each with
+ * its own strides {sequence, token, head} in elements (host arrays of 3; positive
+ * multiples of 8, at least head_dim; head_dim contiguous; 16-byte aligned bases), so a
+ * packed q | k | v buffer or either order of tokens and heads is read in place. dtype 0
+ * f16, 1 bf16; head_dim 64 or 128; heads a multiple of kv_heads: query head h reads key
+ * head h / (heads / kv_heads). scale: finite, not negative.
+ * Returns as the e4m3 linears do; nothing is allocated but the status word. */
+DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
+                                   int dtype, int nseq, int q_len, int k_len, int heads, int kv_heads, int head_dim,
+                                   const int* q_lens, const int* k_lens, int left, int right, int sinks, float scale,
+                                   void* stream);
+
 /* Packs a ggml conv2d weight (ne [KW,KH,IC,OC] f32 == torch [OC][IC][KH][KW]) into
  * the implicit-GEMM layout f16 [OC][KH*KW][icp], icp = IC rounded up to 64. */
 DA3B_API int da3b_pack_conv_weight(const float* w_f32, int OC, int IC, int ksize, void* w_packed, void* stream);
