@@ -1,97 +1,504 @@
 // The e4m3 linear: y = act(x w^T + bias) of rows and weights held as e4m3 with one
 // power-of-two scale for each row and 128 columns of the reduction (fp8.cuh):
 //   y[m][n] = sum_b 2^(ex[m][b] + ew[n][b]) sum_{k in b} qx[m][k] qw[n][k] + bias[n].
+//
+// The scales are applied by the tensor core (tcgen05.mma kind::mxf8f6f4 with ue8m0 block
+// scales): the instruction scales every 32 products, and the four instructions of a block
+// of 128 are given the same scale byte, so the accumulator in tensor memory holds the
+// finished sum and no per-block rescale runs on the CUDA cores.
+//
+// Roles (384 threads, persistent, one CTA or one CTA pair per tile at a time; registers
+// move from the first four warps to the epilogue's, setmaxnreg):
+//   warp 0     TMA: per k-block of 128 bytes the x tile [128][128 B] and the w tile
+//              (128B swizzle) into a ring; with every fourth k-block the scale tiles (512
+//              bytes for 128 rows of four blocks, fp8_scale_offset's order);
+//   warp 1     one thread copies new scale tiles into tensor memory (tcgen05.cp, 32 lanes
+//              x 4 columns, one word = a row's four blocks) and issues four MMAs (K = 32)
+//              a k-block, selecting the block's byte by the descriptor's scale ids;
+//   warps 4-11 epilogue: tensor memory -> registers (128 columns a thread, row = lane) ->
+//              bias, activation, quantisation -> 128-byte rows through a swizzled staging
+//              buffer, so that a store instruction covers four whole 128-byte row pieces.
+// Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
+#include <algorithm>
+#include <atomic>
+#include <cuda.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "act.cuh"
 #include "da3b.h"
 #include "fp8.cuh"
 #include "fp8.h"
 #include "gemm.h"
 #include "ops.h"
+#include "ptx.cuh"
 
 namespace da3b {
 
 namespace {
 
-__device__ __forceinline__ float fp8_value(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+constexpr int kThreads = 384;
+// Launched at 168 registers a thread (64 512 in all): the first warpgroup gives back down
+// to 56, the epilogue's two warpgroups take 224, enough for 128 columns a thread.
+constexpr int kRegsLaunch = 168, kRegsCtl = 56, kRegsEpi = 224;
+static_assert(128 * kRegsCtl + 256 * kRegsEpi <= kThreads * kRegsLaunch, "register split exceeds the launch");
+constexpr int kEpiWarps = 8;
+constexpr int kSfBuffers = 8;  // scale buffers in tensor memory
+
+// CG = 1: a CTA computes 128 x BN, two accumulators, the two halves of the epilogue warps
+// take alternate tiles. CG = 2: a CTA pair computes 256 x 256 (128 x 256 in each CTA's
+// tensor memory), one accumulator, the two halves take 128 columns each: the scales need
+// tensor memory too, so a second 256-column accumulator does not fit.
+template <int CG>
+struct Cfg {
+  static constexpr int kBN = CG == 2 ? 256 : 128;
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kBBytes = 128 * 128;  // each CTA of a pair holds half of the w tile
+  static constexpr int kSfATiles = 1, kSfBTiles = kBN / 128;
+  static constexpr int kSfBytes = 512 * (kSfATiles + kSfBTiles);
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 5;
+  static constexpr int kAcc = CG == 2 ? 1 : 2;
+  static constexpr int kSfCols = 4 * (kSfATiles + kSfBTiles);
+  static constexpr uint32_t kColSf = kAcc * kBN;
+  static constexpr int kEpiBytes = kEpiWarps * (4096 + 2 * 512);  // staging, bias and scale of 128 columns
+  static constexpr int kSmem = 1024 + kStages * (kStageBytes + kSfBytes) + kEpiBytes + 256;
+  static_assert(kColSf + kSfBuffers * kSfCols <= 512, "tensor memory");
+  // A scale buffer is reused kSfBuffers groups later, and a k-block's MMAs start only when
+  // those of the k-block kStages before it are complete, so its readers are done.
+  static_assert(kSfBuffers >= kStages, "scale buffers");
+};
+
+// Instruction descriptor of kind::mxf8f6f4: e4m3 x e4m3, ue8m0 scales, both operands
+// K-major; sf = which byte of the scale words.
+__host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N, int sf) {
+  return (static_cast<uint32_t>(sf) << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(M >> 4) << 24) | (static_cast<uint32_t>(sf) << 29);
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == kActRelu) return v < 0.f ? 0.f : v;  // NaN stays NaN
-  if (act != kActNone) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-  return v;
+template <int CG>
+__device__ __forceinline__ void umma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t accumulate) {
+  if (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
 }
 
-// Reference form: a CTA computes 32 rows x 128 columns, a thread 2 x 8 of them, from
-// dequantised values in shared memory.
-__global__ void __launch_bounds__(256) k_linear_fp8(const Fp8Linear a) {
-  __shared__ float sx[32][33], sw[32][129];
-  const int m0 = blockIdx.y * 32, n0 = blockIdx.x * 128;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int mt = (a.M + 127) / 128, nt = (a.N + 127) / 128;
-  float acc[2][8] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 32) {
-    for (int i = threadIdx.x; i < 32 * 32; i += 256) {
-      const int r = i / 32, c = i % 32, m = m0 + r, k = k0 + c;
-      sx[c][r] = m < a.M && k < a.K ? fp8_value(a.x[static_cast<size_t>(m) * a.ldx + k]) *
-                                          fp8_scale(a.xs[fp8_scale_offset(m, k >> 7, mt)])
-                                    : 0.f;
-    }
-    for (int i = threadIdx.x; i < 128 * 32; i += 256) {
-      const int r = i / 32, c = i % 32, n = n0 + r, k = k0 + c;
-      sw[c][r] = n < a.N && k < a.K ? fp8_value(a.w[static_cast<size_t>(n) * a.ldw + k]) *
-                                          fp8_scale(a.ws[fp8_scale_offset(n, k >> 7, nt)])
-                                    : 0.f;
-    }
-    __syncthreads();
-    for (int c = 0; c < 32; ++c)
+// One 512-byte scale tile from shared memory to 32 lanes x 4 columns, repeated in the four
+// lane quarters. The source is 32 rows of 16 bytes: no swizzle, 128 bytes between groups of
+// eight rows.
+template <int CG>
+__device__ __forceinline__ void copy_sf(uint32_t tmem, uint32_t saddr) {
+  uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  if (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A warp's [32 rows][128 B] piece of the output: lane = row holds 32 words; rows [m0, m0 +
+// 32) and the bytes from column byte cb on of the output. Through the warp's staging buffer
+// (16-byte chunks XOR-swizzled by row), so that eight lanes write 128 consecutive bytes of a
+// row. Where the output is not 16-byte aligned, or at its last columns, element by element.
+// ESZ: bytes an element; RESID: out += value (f32).
+template <int ESZ, bool RESID>
+__device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, const uint32_t (&words)[32], int m0, int n0,
+                                            bool vec, int lane) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+        make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
+  __syncwarp();
+  const int c = lane & 7, n = n0 + c * (16 / ESZ);
+  const bool full = vec && n + 16 / ESZ <= a.N;
+  uint8_t* col = static_cast<uint8_t*>(a.out) + static_cast<size_t>(n) * ESZ;
+  const size_t pitch = static_cast<size_t>(a.ldo) * ESZ;
+  if (full) {
+    uint4 old[8];
+    if (RESID) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(sx[c][ty * 2 + i], sw[c][tx + 16 * j], acc[i][j]);
-    __syncthreads();
+      for (int k = 0; k < 8; ++k) {
+        const int m = m0 + 4 * k + (lane >> 3);
+        if (m < a.M) old[k] = *reinterpret_cast<const uint4*>(col + m * pitch);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int row = 4 * k + (lane >> 3), m = m0 + row;
+      uint4 u = *reinterpret_cast<const uint4*>(stg + row * 128 + ((c ^ (row & 7)) << 4));
+      if (RESID) {
+        u.x = __float_as_uint(__uint_as_float(u.x) + __uint_as_float(old[k].x));
+        u.y = __float_as_uint(__uint_as_float(u.y) + __uint_as_float(old[k].y));
+        u.z = __float_as_uint(__uint_as_float(u.z) + __uint_as_float(old[k].z));
+        u.w = __float_as_uint(__uint_as_float(u.w) + __uint_as_float(old[k].w));
+      }
+      if (m < a.M) *reinterpret_cast<uint4*>(col + m * pitch) = u;
+    }
+  } else if (n < a.N) {
+    const int cnt = min(16 / ESZ, a.N - n);
+    for (int k = 0; k < 8; ++k) {
+      const int row = 4 * k + (lane >> 3), m = m0 + row;
+      if (m >= a.M) break;
+      const uint8_t* src = stg + row * 128 + ((c ^ (row & 7)) << 4);
+      for (int e = 0; e < cnt; ++e) {
+        if (ESZ == 4) {
+          float* o = reinterpret_cast<float*>(col + m * pitch) + e;
+          const float v = reinterpret_cast<const float*>(src)[e];
+          *o = RESID ? *o + v : v;
+        } else if (ESZ == 2) {
+          (reinterpret_cast<uint16_t*>(col + m * pitch))[e] = reinterpret_cast<const uint16_t*>(src)[e];
+        } else {
+          (col + m * pitch)[e] = src[e];
+        }
+      }
+    }
   }
+  __syncwarp();
+}
+
+// Epilogue of a warp's 32 rows x 128 columns held as v (lane = row m0 + lane, column n0 + i).
+// cbias, cscale: the warp's copies of bias and scale for these columns.
+__device__ __forceinline__ void epilogue128(const Fp8Linear& a, float (&v)[128], int m0, int n0, uint8_t* stg,
+                                            const float* cbias, const float* cscale, bool vec, int lane) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int m = m0 + ty * 2 + i;
-    float v[8], amax = 0.f;
+  for (int i = 0; i < 128; i += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(cbias + i);
+    v[i] += b.x;
+    v[i + 1] += b.y;
+    v[i + 2] += b.z;
+    v[i + 3] += b.w;
+  }
+  if (a.act == kActRelu) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int n = n0 + tx + 16 * j;
-      v[j] = n < a.N ? activate(acc[i][j] + (a.bias ? a.bias[n] : 0.f), a.act) : 0.f;
-      amax = fmaxf(amax, finite_abs(v[j]));
+    for (int i = 0; i < 128; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
+  } else if (a.act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < 128; i += 2) {
+      const float2 g = gelu_erf2(make_float2(v[i], v[i + 1]));
+      v[i] = g.x;
+      v[i + 1] = g.y;
     }
+  } else if (a.act == kActGeluR) {
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (m >= a.M) continue;
+    for (int i = 0; i < 128; i += 2) {
+      const float2 g = gelu_r2(make_float2(v[i], v[i + 1]));
+      v[i] = g.x;
+      v[i + 1] = g.y;
+    }
+  }
+  uint32_t words[32];
+  if (a.kind == kFp8OutF16 || a.kind == kFp8OutBF16) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (a.kind == kFp8OutF16) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) words[i] = pack_f16(v[64 * p + 2 * i], v[64 * p + 2 * i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) words[i] = pack_bf16(v[64 * p + 2 * i], v[64 * p + 2 * i + 1]);
+      }
+      store_piece<2, false>(a, stg, words, m0, n0 + 64 * p, vec, lane);
+    }
+  } else if (a.kind == kFp8OutQ) {
+    // the row's 128 columns are one block of the output's scales (n0 is a multiple of 128;
+    // columns past N are zero: their w rows and bias are)
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 128; ++i) amax = fmaxf(amax, n0 + i < a.N ? finite_abs(v[i]) : 0.f);
     const uint32_t byte = fp8_scale_byte(amax);
-    const size_t row = static_cast<size_t>(m) * a.ldo;
-    if (a.kind == kFp8OutQ && tx == 0) a.out_scales[fp8_scale_offset(m, n0 >> 7, mt)] = static_cast<uint8_t>(byte);
+    const float inv = fp8_inv_scale(byte);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n >= a.N) continue;
-      if (a.kind == kFp8OutF16) static_cast<__half*>(a.out)[row + n] = __float2half_rn(v[j]);
-      else if (a.kind == kFp8OutBF16) static_cast<__nv_bfloat16*>(a.out)[row + n] = __float2bfloat16_rn(v[j]);
-      else if (a.kind == kFp8OutF32) static_cast<float*>(a.out)[row + n] = v[j];
-      else if (a.kind == kFp8OutResid) static_cast<float*>(a.out)[row + n] += (a.scale ? a.scale[n] : 1.f) * v[j];
-      else static_cast<uint8_t*>(a.out)[row + n] =
-          static_cast<uint8_t>(fp8_pack4(fp8_nan_if_inf(v[j]) * fp8_inv_scale(byte), 0.f, 0.f, 0.f) & 255u);
+    for (int i = 0; i < 32; ++i)
+      words[i] = fp8_pack4(fp8_nan_if_inf(v[4 * i]) * inv, fp8_nan_if_inf(v[4 * i + 1]) * inv,
+                           fp8_nan_if_inf(v[4 * i + 2]) * inv, fp8_nan_if_inf(v[4 * i + 3]) * inv);
+    if (m0 + lane < a.M && n0 < a.N)
+      a.out_scales[fp8_scale_offset(m0 + lane, n0 >> 7, (a.M + 127) / 128)] = static_cast<uint8_t>(byte);
+    store_piece<1, false>(a, stg, words, m0, n0, vec, lane);
+  } else {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if (a.kind == kFp8OutResid) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[32 * p + i] * cscale[32 * p + i]);
+        store_piece<4, true>(a, stg, words, m0, n0 + 32 * p, vec, lane);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[32 * p + i]);
+        store_piece<4, false>(a, stg, words, m0, n0 + 32 * p, vec, lane);
+      }
     }
+  }
+}
+
+template <int CG>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_fp8_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+               const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+               const __grid_constant__ Fp8Linear a, int vec, int* status) {
+  using C = Cfg<CG>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + C::kStages * C::kABytes;
+  uint8_t* sSf = sB + C::kStages * C::kBBytes;
+  uint8_t* sEpi = sSf + C::kStages * C::kSfBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + C::kEpiBytes);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* tfull = empty + C::kStages;   // [kAcc] accumulator complete
+  uint64_t* tempty = tfull + C::kAcc;     // [kAcc] accumulator read by the epilogue
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + C::kAcc);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+  const int unit = static_cast<int>(blockIdx.x) / CG, units = static_cast<int>(gridDim.x) / CG;
+  const int m_tiles = (a.M + 127) / 128, n_tiles = (a.N + C::kBN - 1) / C::kBN;
+  const int num_tiles = (m_tiles + CG - 1) / CG * n_tiles;
+  const int num_kb = (a.K + 127) / 128;
+  const int row_tiles_n = (a.N + 127) / 128;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < C::kAcc; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], CG == 2 ? 2 * kEpiWarps : 4);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmSA);
+    prefetch_tmap(&tmSB);
+  }
+  if (warp == 1) {
+    if (CG == 2) tmem_alloc2(tmem_slot, 512);
+    else tmem_alloc(tmem_slot, 512);
+  }
+  tc_fence_before();
+  if (CG == 2) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
+  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = unit; t < num_tiles && ok; t += units) {
+        const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, status, kStatusTimeoutEmpty)) { ok = false; break; }
+          const bool sf = (kb & 3) == 0;
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * (C::kStageBytes + (sf ? C::kSfBytes : 0)));
+          uint8_t* da = sA + stage * C::kABytes;
+          uint8_t* db = sB + stage * C::kBBytes;
+          uint8_t* ds = sSf + stage * C::kSfBytes;
+          const int n0 = nt * C::kBN + static_cast<int>(rank) * 128;
+          if (CG == 2) {
+            const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
+            tma2_load_2d(da, &tmA, fb, kb * 128, mt * 128);
+            tma2_load_2d(db, &tmB, fb, kb * 128, n0);
+            if (sf) {
+              tma2_load_2d(ds, &tmSA, fb, 0, (kb >> 2) * m_tiles + mt);
+              tma2_load_2d(ds + 512, &tmSB, fb, 0, (kb >> 2) * row_tiles_n + nt * 2);
+            }
+          } else {
+            tma_load_2d(da, &tmA, &full[stage], kb * 128, mt * 128);
+            tma_load_2d(db, &tmB, &full[stage], kb * 128, n0);
+            if (sf) {
+              tma_load_2d(ds, &tmSA, &full[stage], 0, (kb >> 2) * m_tiles + mt);
+              tma_load_2d(ds + 512, &tmSB, &full[stage], 0, (kb >> 2) * row_tiles_n + nt);
+            }
+          }
+          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int stage = 0, it = 0;
+      uint32_t phase = 0, group = 0;
+      bool ok = true;
+      for (int t = unit; t < num_tiles && ok; t += units, ++it) {
+        const int acc = it % C::kAcc;
+        if (!mbar_wait(&tempty[acc], ((it / C::kAcc) & 1) ^ 1u, status, kStatusTimeoutAccumFree)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * C::kBN;
+        uint32_t sf = 0;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, status, kStatusTimeoutFull)) { ok = false; break; }
+          tc_fence_after();
+          if ((kb & 3) == 0) {
+            sf = tmem + C::kColSf + (group++ % kSfBuffers) * C::kSfCols;
+            const uint32_t ds = smem_u32(sSf + stage * C::kSfBytes);
+#pragma unroll
+            for (int i = 0; i < C::kSfATiles + C::kSfBTiles; ++i) copy_sf<CG>(sf + 4 * i, ds + 512 * i);
+          }
+          const uint64_t ad = umma_desc_sw128(smem_u32(sA + stage * C::kABytes));
+          const uint64_t bd = umma_desc_sw128(smem_u32(sB + stage * C::kBBytes));
+          const uint32_t id = idesc_mxf8(128 * CG, C::kBN, kb & 3);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_mxf8<CG>(d, ad + 2 * k, bd + 2 * k, id, sf, sf + 4, (kb > 0 || k > 0) ? 1u : 0u);
+          if (CG == 2) umma2_commit_mc(&empty[stage], 0x3);
+          else umma_commit(&empty[stage]);
+          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (ok) {
+          if (CG == 2) umma2_commit_mc(&tfull[acc], 0x3);
+          else umma_commit(&tfull[acc]);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* stg = sEpi + (warp - 4) * 4096;
+    float* cbias = reinterpret_cast<float*>(sEpi + kEpiWarps * 4096 + (warp - 4) * 1024);
+    float* cscale = cbias + 128;
+    int it = 0;
+    for (int t = unit; t < num_tiles; t += units, ++it) {
+      const int acc = it % C::kAcc;
+      if (CG == 1 && acc != half) continue;  // the halves take alternate tiles
+      const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
+      const int m0 = mt * 128 + q * 32, n0 = nt * C::kBN + (CG == 2 ? half * 128 : 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + lane + 32 * i;
+        cbias[lane + 32 * i] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+        cscale[lane + 32 * i] = a.scale && n < a.N ? __ldg(a.scale + n) : 1.f;
+      }
+      __syncwarp();
+      if (!mbar_wait_warp(&tfull[acc], (it / C::kAcc) & 1, status, kStatusTimeoutAccum)) break;
+      tc_fence_after();
+      const uint32_t src = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * C::kBN + (CG == 2 ? half * 128 : 0);
+      float v[128];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r[32];
+        tmem_ld32(src + 32 * i, r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[32 * i + j] = __uint_as_float(r[j]);
+      }
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      // the values are in registers: the next tile's MMAs may start
+      if (lane == 0) {
+        if (CG == 2) mbar_arrive_remote_relaxed(mapa_shared(smem_u32(&tempty[acc]), 0));
+        else mbar_arrive(&tempty[acc]);
+      }
+      if (m0 < a.M && n0 < a.N) epilogue128(a, v, m0, n0, stg, cbias, cscale, vec != 0, lane);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // no CTA leaves while its peer may still signal its barriers
+  if (warp == 1) {
+    tc_fence_after();
+    if (CG == 2) tmem_dealloc2(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+int out_size(int kind) { return kind == kFp8OutQ ? 1 : (kind == kFp8OutF16 || kind == kFp8OutBF16) ? 2 : 4; }
+
+int map_codes(CUtensorMap* m, const uint8_t* p, int rows, int K, int ld) {
+  return make_tmap_2d_typed(m, p, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, K, ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Scale tiles as rows of 128 words, `tiles` of them a box.
+int map_scales(CUtensorMap* m, const uint8_t* p, int rows, int K, int tiles) {
+  const int64_t n = static_cast<int64_t>((K + 511) / 512) * ((rows + 127) / 128);
+  if (n > 0x7fffffff) return -2;
+  return make_tmap_2d_typed(m, p, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, static_cast<int>(n), 128, 128, 128, tiles,
+                            CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+int sm_count(int dev) {
+  static std::atomic<int> counts[64];
+  int n = counts[dev & 63].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    counts[dev & 63].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <int CG>
+int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
+  using C = Cfg<CG>;
+  CUtensorMap ta, tb, tsa, tsb;
+  if (map_codes(&ta, a.x, a.M, a.K, a.ldx) || map_codes(&tb, a.w, a.N, a.K, a.ldw) ||
+      map_scales(&tsa, a.xs, a.M, a.K, C::kSfATiles) || map_scales(&tsb, a.ws, a.N, a.K, C::kSfBTiles))
+    return -2;
+  static std::atomic<uint64_t> attr_set{0};  // one bit per device; first calls may race
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((attr_set.load() >> (dev & 63)) & 1)) {
+    if (cudaFuncSetAttribute(k_fp8_gemm<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+      return -3;
+    // the register split waits for registers that the launch must have
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, k_fp8_gemm<CG>) != cudaSuccess ||
+        fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsEpi)
+      return -5;
+    attr_set.fetch_or(uint64_t(1) << (dev & 63));
+  }
+  const long m_units = ((a.M + 127) / 128 + CG - 1) / CG;
+  const long tiles = m_units * ((a.N + C::kBN - 1) / C::kBN);
+  if (tiles > 0x7fffffffL) return -1;
+  const int vec = aligned(a.out, 16) && (static_cast<size_t>(a.ldo) * out_size(a.kind)) % 16 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long>(tiles, sm_count(dev) / CG) * CG));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_fp8_gemm<CG>, ta, tb, tsa, tsb, a, vec, status) == cudaSuccess ? 0 : -4;
+}
+
 }  // namespace
 
 int check_linear_fp8(const Fp8Linear& a) {
-  const uintptr_t osz = a.kind == kFp8OutQ ? 1 : (a.kind == kFp8OutF16 || a.kind == kFp8OutBF16) ? 2 : 4;
   if (a.K <= 0 || a.N <= 0 || a.ldx < a.K || a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.ldo < a.N ||
-      !aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.xs, 16) || !aligned(a.ws, 16) || !aligned(a.out, osz) ||
-      !aligned(a.bias, 4) || !aligned(a.scale, 4))
+      !aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.xs, 16) || !aligned(a.ws, 16) ||
+      !aligned(a.out, out_size(a.kind)) || !aligned(a.bias, 4) || !aligned(a.scale, 4))
     return -1;
   if (a.kind == kFp8OutQ && (a.ldo % 16 || !aligned(a.out, 16) || !aligned(a.out_scales, 16))) return -1;
   return 0;
@@ -99,10 +506,9 @@ int check_linear_fp8(const Fp8Linear& a) {
 
 int linear_fp8(const Fp8Linear& a, int* status, cudaStream_t s) {
   if (a.M == 0) return 0;
-  const dim3 grid((a.N + 127) / 128, (a.M + 31) / 32);
-  (void)status;
-  k_linear_fp8<<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  const long pair_tiles = static_cast<long>((a.M + 255) / 256) * ((a.N + 255) / 256);
+  if (pair_tiles >= 74) return launch<2>(a, status, s);
+  return launch<1>(a, status, s);
 }
 
 }  // namespace da3b
