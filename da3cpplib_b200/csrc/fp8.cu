@@ -18,33 +18,29 @@ namespace da3b {
 namespace {
 
 // 16 consecutive values x[c .. c + 15] of a row as f32, zeros from column K on. VEC: K is
-// a multiple of 16 and the row starts on a 16-byte boundary.
+// a multiple of 16 and the row starts on a 32-byte boundary.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load16(const T* __restrict__ row, int c, int K, float (&v)[16]) {
   if (VEC) {
     if (c < K) {
-      const uint4* p = reinterpret_cast<const uint4*>(row + c);
+      // 32 bytes a load: a warp's loads cover 1024 consecutive bytes
+      uint32_t w[sizeof(T) * 4];
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[8 * i]), "=r"(w[8 * i + 1]), "=r"(w[8 * i + 2]), "=r"(w[8 * i + 3]), "=r"(w[8 * i + 4]),
+                       "=r"(w[8 * i + 5]), "=r"(w[8 * i + 6]), "=r"(w[8 * i + 7])
+                     : "l"(reinterpret_cast<const uint32_t*>(row + c) + 8 * i));
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 u = __ldg(p + i);
-          v[4 * i] = __uint_as_float(u.x);
-          v[4 * i + 1] = __uint_as_float(u.y);
-          v[4 * i + 2] = __uint_as_float(u.z);
-          v[4 * i + 3] = __uint_as_float(u.w);
-        }
+        for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(w[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 u = __ldg(p + i);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            T two[2];
-            *reinterpret_cast<uint32_t*>(two) = w[k];
-            v[8 * i + 2 * k] = static_cast<float>(two[0]);
-            v[8 * i + 2 * k + 1] = static_cast<float>(two[1]);
-          }
+        for (int k = 0; k < 8; ++k) {
+          T two[2];
+          *reinterpret_cast<uint32_t*>(two) = w[k];
+          v[2 * k] = static_cast<float>(two[0]);
+          v[2 * k + 1] = static_cast<float>(two[1]);
         }
       }
     } else {
@@ -58,49 +54,62 @@ __device__ __forceinline__ void load16(const T* __restrict__ row, int c, int K, 
 }
 
 // Codes and scales of the 512 columns [c0, c0 + 512) of row r that a warp holds, 16 a
-// lane (columns c0 + 16 lane ...). Warp-collective.
-__device__ __forceinline__ void store_fp8(const float (&v)[16], int r, int c0, int K, int row_tiles,
-                                          uint8_t* __restrict__ q, int ldq, uint8_t* __restrict__ scales) {
+// lane (columns c0 + 16 lane ...); the scale bytes of the row's blocks from c0 on.
+// Warp-collective. The kernels here are bounded by instructions as much as by memory, so
+// the maximum is taken without looking at infinities (NaN drops out of it by itself) and
+// only a warp that meets one does it again.
+__device__ __forceinline__ void store_fp8(float (&v)[16], int r, int c0, int K, uint8_t* __restrict__ q, int ldq,
+                                          uint8_t* __restrict__ scale4) {
   const int lane = threadIdx.x & 31;
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, finite_abs(v[i]));
+  for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (__any_sync(0xffffffffu, amax > kFltMax)) {
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      amax = fmaxf(amax, finite_abs(v[i]));
+      v[i] = fp8_nan_if_inf(v[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
   const uint32_t byte = fp8_scale_byte(amax);
   const float inv = fp8_inv_scale(byte);
-  float w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = fp8_nan_if_inf(v[i]) * inv;
   const int c = c0 + 16 * lane;
   if (c < K) {  // ldq is a multiple of 16 and at least K
-    uint4 u;
-    u.x = fp8_pack4(w[0], w[1], w[2], w[3]);
-    u.y = fp8_pack4(w[4], w[5], w[6], w[7]);
-    u.z = fp8_pack4(w[8], w[9], w[10], w[11]);
-    u.w = fp8_pack4(w[12], w[13], w[14], w[15]);
-    *reinterpret_cast<uint4*>(q + static_cast<size_t>(r) * ldq + c) = u;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 s2 = make_float2(inv, inv);
+      const float2 a = __fmul2_rn(make_float2(v[4 * i], v[4 * i + 1]), s2);
+      const float2 b = __fmul2_rn(make_float2(v[4 * i + 2], v[4 * i + 3]), s2);
+      w[i] = fp8_pack4(a.x, a.y, b.x, b.y);
+    }
+    *reinterpret_cast<uint4*>(q + static_cast<size_t>(r) * ldq + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  const uint32_t b0 = __shfl_sync(0xffffffffu, byte, 0), b1 = __shfl_sync(0xffffffffu, byte, 8);
-  const uint32_t b2 = __shfl_sync(0xffffffffu, byte, 16), b3 = __shfl_sync(0xffffffffu, byte, 24);
-  if (lane == 0)
-    *reinterpret_cast<uint32_t*>(scales + fp8_scale_offset(r, c0 >> 7, row_tiles)) =
-        b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
+  if ((lane & 7) == 0) scale4[lane >> 3] = static_cast<uint8_t>(byte);
 }
 
+// A warp takes one row and up to two groups of 512 columns of it (blockIdx.y), both loaded
+// before either is worked on.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     k_quantize_fp8(const T* __restrict__ x, int rows, int K, int ldx, uint8_t* __restrict__ q, int ldq,
                    uint8_t* __restrict__ scales) {
-  const int groups = (K + 511) / 512, row_tiles = (rows + 127) / 128;
-  const long items = static_cast<long>(rows) * groups;
-  const long step = static_cast<long>(gridDim.x) * 8;
-  for (long it = static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5); it < items; it += step) {
-    const int r = static_cast<int>(it / groups), c0 = static_cast<int>(it % groups) * 512;
-    float v[16];
-    load16<T, VEC>(x + static_cast<size_t>(r) * ldx, c0 + 16 * (threadIdx.x & 31), K, v);
-    store_fp8(v, r, c0, K, row_tiles, q, ldq, scales);
-  }
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (r >= rows) return;
+  const int row_tiles = (rows + 127) / 128, c0 = blockIdx.y * 1024, lane = threadIdx.x & 31;
+  const T* row = x + static_cast<size_t>(r) * ldx;
+  float v[16], w[16];
+  load16<T, VEC>(row, c0 + 16 * lane, K, v);
+  const bool two = c0 + 512 < K;
+  if (two) load16<T, VEC>(row, c0 + 512 + 16 * lane, K, w);
+  uint8_t* s4 = scales + fp8_scale_offset(r, c0 >> 7, row_tiles);
+  store_fp8(v, r, c0, K, q, ldq, s4);
+  if (two) store_fp8(w, r, c0 + 512, K, q, ldq, s4 + static_cast<size_t>(row_tiles) * 512);
 }
 
 // LayerNorm of f32 rows, two-pass mean and variance in f32 over the row held in
@@ -163,11 +172,12 @@ __global__ void __launch_bounds__(256)
       for (int i = 0; i < 16; ++i)
         y[i] = c + i < K ? (v[j][i] - mean) * rstd * __ldg(g + c + i) + (b ? __ldg(b + c + i) : 0.f) : 0.f;
     }
-    store_fp8(y, r, c0, K, row_tiles, q, ldq, scales);
+    store_fp8(y, r, c0, K, q, ldq, scales + fp8_scale_offset(r, c0 >> 7, row_tiles));
   }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 bool bad_codes(const uint8_t* q, int ldq, const uint8_t* scales, int K) {
   return ldq < K || ldq % 16 || !aligned16(q) || !aligned16(scales);
@@ -177,12 +187,12 @@ template <typename T>
 int launch_quantize(const void* xv, int rows, int K, int ldx, uint8_t* q, int ldq, uint8_t* scales, cudaStream_t s) {
   const T* x = static_cast<const T*>(xv);
   if (reinterpret_cast<uintptr_t>(x) % sizeof(T)) return -1;
-  const long items = static_cast<long>(rows) * ((K + 511) / 512);
-  const unsigned blocks = static_cast<unsigned>(std::min<long>((items + 7) / 8, 148L * 64));
-  if (K % 16 == 0 && (static_cast<size_t>(ldx) * sizeof(T)) % 16 == 0 && aligned16(x))
-    k_quantize_fp8<T, true><<<blocks, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
+  const dim3 grid((static_cast<unsigned>(rows) + 7) / 8, (static_cast<unsigned>(K) + 1023) / 1024);
+  if (grid.y > 65535) return -1;
+  if (K % 16 == 0 && (static_cast<size_t>(ldx) * sizeof(T)) % 32 == 0 && aligned32(x))
+    k_quantize_fp8<T, true><<<grid, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
   else
-    k_quantize_fp8<T, false><<<blocks, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
+    k_quantize_fp8<T, false><<<grid, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
@@ -206,7 +216,7 @@ int layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g, cons
   if (reinterpret_cast<uintptr_t>(x) % 4 || reinterpret_cast<uintptr_t>(g) % 4 || reinterpret_cast<uintptr_t>(b) % 4)
     return -1;
   if (rows == 0) return 0;
-  const bool vec = K % 16 == 0 && ldx % 4 == 0 && aligned16(x) && aligned16(g) && aligned16(b);
+  const bool vec = K % 16 == 0 && ldx % 8 == 0 && aligned32(x) && aligned32(g) && aligned32(b);
   const unsigned per_warp = static_cast<unsigned>((rows + 7) / 8), per_block = static_cast<unsigned>(rows);
 #define DA3B_LNF8(W, NV, GRID)                                                                          \
   do {                                                                                                  \

@@ -7,7 +7,7 @@
 // of 128 are given the same scale byte, so the accumulator in tensor memory holds the
 // finished sum and no per-block rescale runs on the CUDA cores.
 //
-// Roles (384 threads, persistent, one CTA or one CTA pair per tile at a time; registers
+// Roles (640 threads, persistent, one CTA or one CTA pair per tile at a time; registers
 // move from the first four warps to the epilogue's, setmaxnreg):
 //   warp 0     TMA: per k-block of 128 bytes the x tile [128][128 B] and the w tile
 //              (128B swizzle) into a ring; with every fourth k-block the scale tiles (512
@@ -15,9 +15,11 @@
 //   warp 1     one thread copies new scale tiles into tensor memory (tcgen05.cp, 32 lanes
 //              x 4 columns, one word = a row's four blocks) and issues four MMAs (K = 32)
 //              a k-block, selecting the block's byte by the descriptor's scale ids;
-//   warps 4-11 epilogue: tensor memory -> registers (128 columns a thread, row = lane) ->
-//              bias, activation, quantisation -> 128-byte rows through a swizzled staging
-//              buffer, so that a store instruction covers four whole 128-byte row pieces.
+//   warps 4-19 epilogue: tensor memory -> registers (64 columns a thread, row = lane) ->
+//              bias, activation, quantisation -> 64-byte row pieces through a swizzled
+//              staging buffer, so that four lanes store consecutive bytes of a row. Four
+//              warps an SM sub-partition hide each other's latencies: with eight warps of
+//              128 columns, M = 87680, K = 1024, N = 4096 with GELU took 528-580 us.
 // Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
 #include <algorithm>
 #include <atomic>
@@ -38,17 +40,19 @@ namespace da3b {
 
 namespace {
 
-constexpr int kThreads = 384;
-// Launched at 168 registers a thread (64 512 in all): the first warpgroup gives back down
-// to 56, the epilogue's two warpgroups take 224, enough for 128 columns a thread.
-constexpr int kRegsLaunch = 168, kRegsCtl = 56, kRegsEpi = 224;
-static_assert(128 * kRegsCtl + 256 * kRegsEpi <= kThreads * kRegsLaunch, "register split exceeds the launch");
-constexpr int kEpiWarps = 8;
+constexpr int kThreads = 640;
+// Launched at 96 registers a thread (61 440 in all): the first warpgroup gives back down to
+// 40, the epilogue's four warpgroups take 104.
+constexpr int kRegsLaunch = 96, kRegsCtl = 40, kRegsEpi = 104;
+static_assert(128 * kRegsCtl + 512 * kRegsEpi <= kThreads * kRegsLaunch, "register split exceeds the launch");
+constexpr int kEpiWarps = 16;
+constexpr int kStageOut = 2048;                  // a warp's staging buffer, [32 rows][64 B]
+constexpr int kEpiWarpBytes = kStageOut + 3 * 256;  // + bias and scale of 64 columns, 32 maxima (x 2)
 constexpr int kSfBuffers = 8;  // scale buffers in tensor memory
 
-// CG = 1: a CTA computes 128 x BN, two accumulators, the two halves of the epilogue warps
+// CG = 1: a CTA computes 128 x 128, two accumulators, the two halves of the epilogue warps
 // take alternate tiles. CG = 2: a CTA pair computes 256 x 256 (128 x 256 in each CTA's
-// tensor memory), one accumulator, the two halves take 128 columns each: the scales need
+// tensor memory), one accumulator that all epilogue warps read at once: the scales need
 // tensor memory too, so a second 256-column accumulator does not fit.
 template <int CG>
 struct Cfg {
@@ -62,7 +66,7 @@ struct Cfg {
   static constexpr int kAcc = CG == 2 ? 1 : 2;
   static constexpr int kSfCols = 4 * (kSfATiles + kSfBTiles);
   static constexpr uint32_t kColSf = kAcc * kBN;
-  static constexpr int kEpiBytes = kEpiWarps * (4096 + 2 * 512);  // staging, bias and scale of 128 columns
+  static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
   static constexpr int kSmem = 1024 + kStages * (kStageBytes + kSfBytes) + kEpiBytes + 256;
   static_assert(kColSf + kSfBuffers * kSfCols <= 512, "tensor memory");
   // A scale buffer is reused kSfBuffers groups later, and a k-block's MMAs start only when
@@ -109,6 +113,46 @@ __device__ __forceinline__ void copy_sf(uint32_t tmem, uint32_t saddr) {
   else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
 }
 
+// Erf-form GELU v Phi(v) of eight values, Phi(v) = 1 / (1 + 2^(-v Q(v^2))): Q is a
+// degree-6 polynomial fitted (Lawson-weighted least squares towards the minimax) to the
+// logit of the normal distribution function on |v| <= 6 so that |v Phi(v)| is off by at most
+// 6.8e-8; beyond 6, v^2 is held at 36 and Phi is 0 or 1 to 1e-9. Ten multiply-adds and two
+// MUFU operations a value; the four pairs run side by side, because a chain of about
+// fifteen dependent operations a value otherwise leaves the pipes idle (the M = 87680,
+// K = 1024, N = 4096 product with GELU took 723 us with one chain at a time).
+__device__ __forceinline__ void gelu8(float* v) {
+  float2 x[4], q[4];
+  const float2 one = make_float2(1.f, 1.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 w = make_float2(v[2 * i], v[2 * i + 1]);
+    x[i] = __fmul2_rn(w, w);
+    x[i] = make_float2(fminf(x[i].x, 36.f), fminf(x[i].y, 36.f));
+  }
+  auto step = [&](float c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __ffma2_rn(q[i], x[i], make_float2(c, c));
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = __ffma2_rn(make_float2(-5.209905840e-09f, -5.209905840e-09f), x[i], make_float2(3.850448707e-07f, 3.850448707e-07f));
+  step(-1.145242732e-05f);
+  step(1.593893976e-04f);
+  step(9.559298633e-05f);
+  step(-0.1048385799f);
+  step(-2.302207232f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 u = __fmul2_rn(q[i], make_float2(v[2 * i], v[2 * i + 1]));
+    const float2 d = __fadd2_rn(make_float2(ex2_approx(u.x), ex2_approx(u.y)), one);
+    float rx, ry;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rx) : "f"(d.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ry) : "f"(d.y));
+    v[2 * i] *= rx;
+    v[2 * i + 1] *= ry;
+  }
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -118,36 +162,35 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A warp's [32 rows][128 B] piece of the output: lane = row holds 32 words; rows [m0, m0 +
-// 32) and the bytes from column byte cb on of the output. Through the warp's staging buffer
-// (16-byte chunks XOR-swizzled by row), so that eight lanes write 128 consecutive bytes of a
-// row. Where the output is not 16-byte aligned, or at its last columns, element by element.
+// A warp's [32 rows][64 B] piece of the output: lane = row holds 16 words; rows [m0, m0 +
+// 32), columns from n0 on. Through the warp's staging buffer (16-byte chunks XOR-swizzled
+// by row), so that four lanes write 64 consecutive bytes of a row. Where the output is not
+// 16-byte aligned, or at its last columns, element by element.
 // ESZ: bytes an element; RESID: out += value (f32).
 template <int ESZ, bool RESID>
-__device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, const uint32_t (&words)[32], int m0, int n0,
+__device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, const uint32_t (&words)[16], int m0, int n0,
                                             bool vec, int lane) {
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    *reinterpret_cast<uint4*>(stg + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(stg + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
         make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
   __syncwarp();
-  const int c = lane & 7, n = n0 + c * (16 / ESZ);
-  const bool full = vec && n + 16 / ESZ <= a.N;
-  uint8_t* col = static_cast<uint8_t*>(a.out) + static_cast<size_t>(n) * ESZ;
+  const int c = lane & 3, n = n0 + c * (16 / ESZ);
   const size_t pitch = static_cast<size_t>(a.ldo) * ESZ;
-  if (full) {
-    uint4 old[8];
+  if (vec && n + 16 / ESZ <= a.N) {
+    uint8_t* col = static_cast<uint8_t*>(a.out) + static_cast<size_t>(n) * ESZ;
+    uint4 old[4];
     if (RESID) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int m = m0 + 4 * k + (lane >> 3);
+      for (int k = 0; k < 4; ++k) {
+        const int m = m0 + 8 * k + (lane >> 2);
         if (m < a.M) old[k] = *reinterpret_cast<const uint4*>(col + m * pitch);
       }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int row = 4 * k + (lane >> 3), m = m0 + row;
-      uint4 u = *reinterpret_cast<const uint4*>(stg + row * 128 + ((c ^ (row & 7)) << 4));
+    for (int k = 0; k < 4; ++k) {
+      const int row = 8 * k + (lane >> 2), m = m0 + row;
+      uint4 u = *reinterpret_cast<const uint4*>(stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
       if (RESID) {
         u.x = __float_as_uint(__uint_as_float(u.x) + __uint_as_float(old[k].x));
         u.y = __float_as_uint(__uint_as_float(u.y) + __uint_as_float(old[k].y));
@@ -156,21 +199,28 @@ __device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, co
       }
       if (m < a.M) *reinterpret_cast<uint4*>(col + m * pitch) = u;
     }
-  } else if (n < a.N) {
-    const int cnt = min(16 / ESZ, a.N - n);
-    for (int k = 0; k < 8; ++k) {
-      const int row = 4 * k + (lane >> 3), m = m0 + row;
-      if (m >= a.M) break;
-      const uint8_t* src = stg + row * 128 + ((c ^ (row & 7)) << 4);
-      for (int e = 0; e < cnt; ++e) {
+  }
+  // every 16-byte chunk was stored above, or is stored here element by element, 32
+  // consecutive elements a store
+  const int n_vec = vec ? a.N / (16 / ESZ) * (16 / ESZ) : 0;
+  if (n0 + 64 / ESZ > n_vec) {
+    const int rows = min(32, a.M - m0);
+    uint8_t* out = static_cast<uint8_t*>(a.out) + m0 * pitch;
+#pragma unroll 4
+    for (int row = 0; row < rows; ++row) {
+#pragma unroll
+      for (int e = lane; e < 64 / ESZ; e += 32) {
+        const int ne = n0 + e, b = e * ESZ;
+        if (ne < n_vec || ne >= a.N) continue;
+        const uint8_t* src = stg + row * 64 + (((b >> 4) ^ ((row >> 1) & 3)) << 4) + (b & 15);
+        uint8_t* o = out + row * pitch + static_cast<size_t>(ne) * ESZ;
         if (ESZ == 4) {
-          float* o = reinterpret_cast<float*>(col + m * pitch) + e;
-          const float v = reinterpret_cast<const float*>(src)[e];
-          *o = RESID ? *o + v : v;
+          const float v = *reinterpret_cast<const float*>(src);
+          *reinterpret_cast<float*>(o) = RESID ? *reinterpret_cast<const float*>(o) + v : v;
         } else if (ESZ == 2) {
-          (reinterpret_cast<uint16_t*>(col + m * pitch))[e] = reinterpret_cast<const uint16_t*>(src)[e];
+          *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(src);
         } else {
-          (col + m * pitch)[e] = src[e];
+          *o = *src;
         }
       }
     }
@@ -178,13 +228,17 @@ __device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, co
   __syncwarp();
 }
 
-// Epilogue of a warp's 32 rows x 128 columns held as v (lane = row m0 + lane, column n0 + i).
-// cbias, cscale: the warp's copies of bias and scale for these columns.
-__device__ __forceinline__ void epilogue128(const Fp8Linear& a, float (&v)[128], int m0, int n0, uint8_t* stg,
-                                            const float* cbias, const float* cscale, bool vec, int lane) {
+// Epilogue of a warp's 32 rows x 64 columns held as v (lane = row m0 + lane, column n0 + i).
+// ctab: the warp's copies of bias and scale for these columns, [2][64], and the row maxima
+// it shares with the warp that has the other 64 columns of the block, [2][32]: `other` is
+// that warp's table, `pair` the barrier of the two, `flip` alternates with the tiles. False if
+// a wait ran out.
+__device__ __forceinline__ bool epilogue64(const Fp8Linear& a, float (&v)[64], int m0, int n0, uint8_t* stg, float* ctab,
+                                           const float* other, uint64_t* pair, uint32_t flip, bool vec, int lane,
+                                           int* status) {
 #pragma unroll
-  for (int i = 0; i < 128; i += 4) {
-    const float4 b = *reinterpret_cast<const float4*>(cbias + i);
+  for (int i = 0; i < 64; i += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(ctab + i);
     v[i] += b.x;
     v[i + 1] += b.y;
     v[i + 2] += b.z;
@@ -192,48 +246,42 @@ __device__ __forceinline__ void epilogue128(const Fp8Linear& a, float (&v)[128],
   }
   if (a.act == kActRelu) {
 #pragma unroll
-    for (int i = 0; i < 128; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
-  } else if (a.act == kActGelu) {
+    for (int i = 0; i < 64; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
+  } else if (a.act != kActNone) {
 #pragma unroll
-    for (int i = 0; i < 128; i += 2) {
-      const float2 g = gelu_erf2(make_float2(v[i], v[i + 1]));
-      v[i] = g.x;
-      v[i + 1] = g.y;
-    }
-  } else if (a.act == kActGeluR) {
-#pragma unroll
-    for (int i = 0; i < 128; i += 2) {
-      const float2 g = gelu_r2(make_float2(v[i], v[i + 1]));
-      v[i] = g.x;
-      v[i + 1] = g.y;
-    }
+    for (int i = 0; i < 64; i += 8) gelu8(v + i);
   }
-  uint32_t words[32];
+  uint32_t words[16];
   if (a.kind == kFp8OutF16 || a.kind == kFp8OutBF16) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       if (a.kind == kFp8OutF16) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) words[i] = pack_f16(v[64 * p + 2 * i], v[64 * p + 2 * i + 1]);
+        for (int i = 0; i < 16; ++i) words[i] = pack_f16(v[32 * p + 2 * i], v[32 * p + 2 * i + 1]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) words[i] = pack_bf16(v[64 * p + 2 * i], v[64 * p + 2 * i + 1]);
+        for (int i = 0; i < 16; ++i) words[i] = pack_bf16(v[32 * p + 2 * i], v[32 * p + 2 * i + 1]);
       }
-      store_piece<2, false>(a, stg, words, m0, n0 + 64 * p, vec, lane);
+      store_piece<2, false>(a, stg, words, m0, n0 + 32 * p, vec, lane);
     }
   } else if (a.kind == kFp8OutQ) {
-    // the row's 128 columns are one block of the output's scales (n0 is a multiple of 128;
-    // columns past N are zero: their w rows and bias are)
+    // this warp's 64 columns and its partner's are one block of the output's scales;
+    // columns past N are zero (w has no rows there, and their bias is zero)
     float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 128; ++i) amax = fmaxf(amax, n0 + i < a.N ? finite_abs(v[i]) : 0.f);
+    for (int i = 0; i < 64; ++i) amax = fmaxf(amax, finite_abs(v[i]));
+    ctab[128 + 32 * flip + lane] = amax;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(pair);
+    if (!mbar_wait_warp(pair, flip, status, kStatusTimeoutAccum)) return false;
+    amax = fmaxf(amax, other[128 + 32 * flip + lane]);
     const uint32_t byte = fp8_scale_byte(amax);
     const float inv = fp8_inv_scale(byte);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 16; ++i)
       words[i] = fp8_pack4(fp8_nan_if_inf(v[4 * i]) * inv, fp8_nan_if_inf(v[4 * i + 1]) * inv,
                            fp8_nan_if_inf(v[4 * i + 2]) * inv, fp8_nan_if_inf(v[4 * i + 3]) * inv);
-    if (m0 + lane < a.M && n0 < a.N)
+    if (m0 + lane < a.M && (n0 & 127) == 0)
       a.out_scales[fp8_scale_offset(m0 + lane, n0 >> 7, (a.M + 127) / 128)] = static_cast<uint8_t>(byte);
     store_piece<1, false>(a, stg, words, m0, n0, vec, lane);
   } else {
@@ -241,15 +289,16 @@ __device__ __forceinline__ void epilogue128(const Fp8Linear& a, float (&v)[128],
     for (int p = 0; p < 4; ++p) {
       if (a.kind == kFp8OutResid) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[32 * p + i] * cscale[32 * p + i]);
-        store_piece<4, true>(a, stg, words, m0, n0 + 32 * p, vec, lane);
+        for (int i = 0; i < 16; ++i) words[i] = __float_as_uint(v[16 * p + i] * ctab[64 + 16 * p + i]);
+        store_piece<4, true>(a, stg, words, m0, n0 + 16 * p, vec, lane);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) words[i] = __float_as_uint(v[32 * p + i]);
-        store_piece<4, false>(a, stg, words, m0, n0 + 32 * p, vec, lane);
+        for (int i = 0; i < 16; ++i) words[i] = __float_as_uint(v[16 * p + i]);
+        store_piece<4, false>(a, stg, words, m0, n0 + 16 * p, vec, lane);
       }
     }
   }
+  return true;
 }
 
 template <int CG>
@@ -268,7 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* empty = full + C::kStages;
   uint64_t* tfull = empty + C::kStages;   // [kAcc] accumulator complete
   uint64_t* tempty = tfull + C::kAcc;     // [kAcc] accumulator read by the epilogue
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + C::kAcc);
+  uint64_t* pairs = tempty + C::kAcc;     // [8] row maxima of both warps of a block written
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pairs + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
@@ -285,8 +335,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < C::kAcc; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], CG == 2 ? 2 * kEpiWarps : 4);
+      mbar_init(&tempty[i], CG == 2 ? 2 * kEpiWarps : kEpiWarps / 2);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&pairs[i], 2);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -303,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
-  else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
@@ -378,30 +429,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {
-    const int q = warp & 3, half = (warp - 4) >> 2;
-    uint8_t* stg = sEpi + (warp - 4) * 4096;
-    float* cbias = reinterpret_cast<float*>(sEpi + kEpiWarps * 4096 + (warp - 4) * 1024);
-    float* cscale = cbias + 128;
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter, 64-column part of the tile
+    const int cols = (CG == 2 ? part : part & 1) * 64;
+    uint8_t* stg = sEpi + (warp - 4) * kEpiWarpBytes;
+    float* ctab = reinterpret_cast<float*>(stg + kStageOut);
+    // the warp with the other half of a 128-column block: the next or last part
+    const float* other = reinterpret_cast<const float*>(sEpi + ((warp - 4) ^ 4) * kEpiWarpBytes + kStageOut);
+    uint64_t* pair = &pairs[q + 4 * (part >> 1)];
+    uint32_t uses = 0;
     int it = 0;
     for (int t = unit; t < num_tiles; t += units, ++it) {
       const int acc = it % C::kAcc;
-      if (CG == 1 && acc != half) continue;  // the halves take alternate tiles
+      if (CG == 1 && acc != part >> 1) continue;  // the halves take alternate tiles
       const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
-      const int m0 = mt * 128 + q * 32, n0 = nt * C::kBN + (CG == 2 ? half * 128 : 0);
+      const int m0 = mt * 128 + q * 32, n0 = nt * C::kBN + cols;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         const int n = n0 + lane + 32 * i;
-        cbias[lane + 32 * i] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
-        cscale[lane + 32 * i] = a.scale && n < a.N ? __ldg(a.scale + n) : 1.f;
+        ctab[lane + 32 * i] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
+        ctab[64 + lane + 32 * i] = a.scale && n < a.N ? __ldg(a.scale + n) : 1.f;
       }
       __syncwarp();
       if (!mbar_wait_warp(&tfull[acc], (it / C::kAcc) & 1, status, kStatusTimeoutAccum)) break;
       tc_fence_after();
-      const uint32_t src = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * C::kBN + (CG == 2 ? half * 128 : 0);
-      float v[128];
+      const uint32_t src = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * C::kBN + cols;
+      float v[64];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t r[32];
         tmem_ld32(src + 32 * i, r);
 #pragma unroll
@@ -415,7 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (CG == 2) mbar_arrive_remote_relaxed(mapa_shared(smem_u32(&tempty[acc]), 0));
         else mbar_arrive(&tempty[acc]);
       }
-      if (m0 < a.M && n0 < a.N) epilogue128(a, v, m0, n0, stg, cbias, cscale, vec != 0, lane);
+      // whole 128-column blocks are in or out together, so both warps of a pair come here
+      if (m0 < a.M && (n0 & ~127) < a.N &&
+          !epilogue64(a, v, m0, n0, stg, ctab, other, pair, uses++ & 1, vec != 0, lane, status))
+        break;
     }
   }
 

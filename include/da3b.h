@@ -217,7 +217,7 @@ DA3B_API int da3b_layernorm_fp8(const float* x, int rows, int K, int ldx, const 
                                 float eps, void* q, int ldq, void* scales, void* stream);
 
 /* y = act(x w^T + bias) of quantised x [M][K] and w [N][K]; bias f32 [N] or NULL, act as
- * da3b_linear_f16, sums in f32.
+ * da3b_linear_f16 (2 and 3 are the same erf-form GELU here), sums in f32.
  *   da3b_linear_fp8:           y [M][ldo] of type out_dtype.
  *   da3b_linear_fp8_q:         y quantised by the product's epilogue: codes out_q [M][ldo]
  *                              (ldo a multiple of 16, columns from N on untouched) and
