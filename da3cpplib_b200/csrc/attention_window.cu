@@ -4,6 +4,8 @@
 // (the queries are the last ones of the keys) and sees the keys j < kl with
 // j <= p + right and (j >= p - left or j < sinks). o = sum_j softmax_j(scale q.k_j) v_j; a
 // query that sees nothing gets zeros, rows from ql on are not written.
+#include <atomic>
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -60,10 +62,481 @@ __global__ void __launch_bounds__(256) k_attn_window(const AttnWindow a) {
   for (int e = 0; e < E; ++e) out[e] = static_cast<T>(l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l));
 }
 
+
+// ------------------------------------------------------------------ many queries
+// Two tiles of 128 query rows a CTA (one CTA per SM, 12 warps), key tiles of 128 shared by
+// both. A query row is one (token, head): g query heads that share a key head lie side by
+// side, 128 / g tokens a tile, so that shared heads read their keys once and a tile spans
+// few positions (a window's ends are masked work).
+//   warp 0     TMA: both Q tiles, then the key tiles that some row sees, K and V each in a
+//              ring of its own ([128 keys][64 dims] boxes, 128B swizzle);
+//   warp 1     one thread issues S_t = Q_t K^T (M = N = 128) and O_t += P_t V (P_t from
+//              tensor memory; V is read as it lies, its dims contiguous: an MN-major operand);
+//   warps 4-7  softmax of query tile 0, warps 8-11 of tile 1: thread = row (its TMEM lane),
+//              the row's 128 scores in registers, one pass; P back to tensor memory.
+// Tensor memory (512 columns): head_dim 64: S_t 128, P_t 64, O_t 64 columns each, so S_t of
+// the next key tile is issued as soon as the scores are in registers, while their
+// exponentials are taken. head_dim 128: O_t takes 128 columns and P_t lies over S_t, so
+// S_t of the next tile follows the P V product of this one.
+// The maximum of a row is raised only when a tile exceeds it by more than 2^8; O_t is then
+// rescaled in tensor memory. Sums are f32 of the unrounded probabilities.
+// Masks are applied to the tiles that a window's end, the sinks' end or the last key cuts.
+// V rows of such tiles that no row of the CTA sees are zeroed in shared memory (0 * NaN).
+
+constexpr int kKT = 128;                // keys per tile
+constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the row's maximum
+constexpr int kThreads = 384;
+constexpr int kRegsLaunch = 168, kRegsCtl = 56, kRegsSoft = 224;
+static_assert(128 * kRegsCtl + 256 * kRegsSoft <= kThreads * kRegsLaunch, "register split exceeds the launch");
+
+template <int D>
+struct WinCfg {
+  static constexpr bool kAlias = D == 128;      // P over S
+  static constexpr int kTile = 128 * D * 2;     // bytes of a Q, K or V tile
+  static constexpr int kRing = D == 64 ? 4 : 2; // K tiles and V tiles in flight
+  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kRing * kTile + 256;
+  static constexpr uint32_t kColS = 0, kColP = kAlias ? 0 : 256, kStepP = kAlias ? 128 : 64;
+  static constexpr uint32_t kColO = kAlias ? 256 : 384;
+};
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe (the MUFU pipe takes one exponential a score
+// otherwise, and bounds the kernel): x = j + f with j = round(x) (adding 1.5 * 2^23 leaves j
+// in the low mantissa bits), f in [-0.5, 0.5]; 2^f by a cubic fitted to relative error
+// (max 7.5e-5, below the rounding of P to 16 bits); j is added to the exponent field. x is
+// held at -125, where the result rounds to 0 in f16 and to 2^-125 in bf16 (at most 2^-117 of
+// the row's largest probability).
+__device__ __forceinline__ float2 exp2_cubic(float2 x) {
+  constexpr float kShift = 12582912.0f;
+  constexpr float c3 = 0.05517166853f, c2 = 0.24261112511f, c1 = 0.69326096773f, c0 = 0.99992805719f;
+  x = make_float2(fmax_nan(x.x, -125.0f), fmax_nan(x.y, -125.0f));
+  const float2 t = __fadd2_rn(x, make_float2(kShift, kShift));
+  const float2 j = __fadd2_rn(t, make_float2(-kShift, -kShift));
+  const float2 f = __fadd2_rn(x, make_float2(-j.x, -j.y));
+  float2 p = __ffma2_rn(make_float2(c3, c3), f, make_float2(c2, c2));
+  p = __ffma2_rn(p, f, make_float2(c1, c1));
+  p = __ffma2_rn(p, f, make_float2(c0, c0));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// Shared-memory descriptor of an MN-major operand tile in 128B-swizzled rows of 64 values:
+// 1024 bytes between groups of eight k rows, lbo bytes between 64-wide column chunks.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// What the rows of one query tile see: tokens [i0, i0 + n) of a sequence at positions from
+// p on.
+struct Span {
+  int n;                 // tokens inside the sequence (0: the tile has no rows)
+  int hi_min, hi_max;    // last visible key of its first and last row
+  int lo_min, lo_max;    // first key of their windows
+  __device__ Span(int i0, int tokens, int ql, int kl, int left, int right) {
+    n = min(max(ql - i0, 0), tokens);
+    const int p = kl - ql + i0, pl = p + max(n - 1, 0);
+    hi_min = min(kl - 1, p + right);
+    hi_max = min(kl - 1, pl + right);
+    lo_min = max(0, p - left);
+    lo_max = max(0, pl - left);
+  }
+  __device__ bool sees(int k0, int sinks) const {  // some key of [k0, k0 + 128)
+    return n > 0 && k0 <= hi_max && (k0 + kKT > lo_min || k0 < sinks);
+  }
+  __device__ bool whole(int k0, int sinks) const {  // every row sees every key of the tile
+    return k0 + kKT - 1 <= hi_min && (k0 >= lo_max || k0 + kKT <= sinks);
+  }
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnWindow a, int g, int tokens,
+                 int tiles, int* status) {
+  using C = WinCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                       // [2] tiles
+  uint8_t* sK = sQ + 2 * C::kTile;          // [kRing]
+  uint8_t* sV = sK + C::kRing * C::kTile;   // [kRing]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + C::kRing * C::kTile);
+  uint64_t* k_full = q_full + 1;            // [kRing] each
+  uint64_t* k_empty = k_full + C::kRing;
+  uint64_t* v_full = k_empty + C::kRing;
+  uint64_t* v_empty = v_full + C::kRing;
+  uint64_t* s_full = v_empty + C::kRing;    // [2] S_t complete
+  uint64_t* s_free = s_full + 2;            // [2] S_t in registers (4 warps)
+  uint64_t* p_ready = s_free + 2;           // [2] P_t written, O_t rescaled, V rows zeroed (4 warps)
+  uint64_t* pv_done = p_ready + 2;          // [2] P_t V complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile2 = static_cast<int>(blockIdx.x) % tiles;
+  const int hg = static_cast<int>(blockIdx.x) / tiles % (a.heads / g);
+  const int b = static_cast<int>(blockIdx.x) / tiles / (a.heads / g);
+  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
+  const int i0 = tile2 * 2 * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
+  if (i0 >= ql) return;
+  const Span sp[2] = {Span(i0, tokens, ql, kl, a.left, a.right), Span(i0 + tokens, tokens, ql, kl, a.left, a.right)};
+  // key tiles of the CTA: n_sink from the front, then those of the windows
+  const int hi = sp[1].n > 0 ? sp[1].hi_max : sp[0].hi_max, lo = sp[0].lo_min;
+  const int w0 = lo / kKT;
+  const int n_sink = hi < 0 ? 0 : min(w0, (min(a.sinks, hi + 1) + kKT - 1) / kKT);
+  const int n_all = hi < 0 ? 0 : n_sink + hi / kKT - w0 + 1;
+  auto key0 = [&](int n) { return (n < n_sink ? n : w0 + n - n_sink) * kKT; };
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < C::kRing; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&p_ready[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
+    if (warp == 0) {
+      if (lane == 0 && n_all > 0) {
+        const int nt = sp[1].n > 0 ? 2 : 1;
+        const uint32_t q_bytes = static_cast<uint32_t>(g * tokens) * 128;  // of one 64-wide box
+        mbar_arrive_expect_tx(q_full, q_bytes * (D / 64) * nt);
+        for (int t = 0; t < nt; ++t)
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(sQ + t * C::kTile + c * 16384, &tmQ, q_full, c * 64, h0, i0 + t * tokens, b);
+        for (int n = 0; n < n_all; ++n) {
+          const int st = n % C::kRing;
+          const uint32_t par = ((n / C::kRing) & 1) ^ 1u;
+          if (!mbar_wait(&k_empty[st], par, status, kStatusTimeoutEmpty)) break;
+          mbar_arrive_expect_tx(&k_full[st], C::kTile);
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(sK + st * C::kTile + c * 16384, &tmK, &k_full[st], c * 64, hk, key0(n), b);
+          if (!mbar_wait(&v_empty[st], par, status, kStatusTimeoutEmpty)) break;
+          mbar_arrive_expect_tx(&v_full[st], C::kTile);
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(sV + st * C::kTile + c * 16384, &tmV, &v_full[st], c * 64, hk, key0(n), b);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0 && n_all > 0) {
+        constexpr uint32_t fmt = BF16 ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t id_s = umma_idesc_f16(128, kKT) | fmt;
+        constexpr uint32_t id_o = umma_idesc_f16(128, D) | fmt | (1u << 16);  // B is MN-major
+        int ns[2] = {0, 0}, np[2] = {0, 0};  // S and P V products issued
+        bool ok = mbar_wait(q_full, 0, status, kStatusTimeoutFull);
+        auto wait_k = [&](int n) { return mbar_wait(&k_full[n % C::kRing], (n / C::kRing) & 1, status, kStatusTimeoutFull); };
+        auto issue_s = [&](int t, int n) -> bool {
+          if (!C::kAlias && ns[t] > 0 &&
+              !mbar_wait(&s_free[t], (ns[t] - 1) & 1, status, kStatusTimeoutAccumFree))
+            return false;
+          tc_fence_after();
+          const uint32_t q = smem_u32(sQ + t * C::kTile), k = smem_u32(sK + n % C::kRing * C::kTile);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint64_t qd = umma_desc_sw128(q + c * 16384), kd = umma_desc_sw128(k + c * 16384);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(tmem + C::kColS + t * 128, qd + 2 * kk, kd + 2 * kk, id_s, (c > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&s_full[t]);
+          ++ns[t];
+          return true;
+        };
+        auto issue_pv = [&](int t, int n) -> bool {
+          if (!mbar_wait(&p_ready[t], np[t] & 1, status, kStatusTimeoutFull)) return false;
+          tc_fence_after();
+          const uint64_t vd = desc_mn_sw128(smem_u32(sV + n % C::kRing * C::kTile), 16384);
+#pragma unroll
+          for (int kk = 0; kk < kKT / 16; ++kk)
+            umma_f16_tmem_a(tmem + C::kColO + t * D, tmem + C::kColP + t * C::kStepP + 8 * kk, vd + 128 * kk, id_o,
+                            (np[t] > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&pv_done[t]);
+          ++np[t];
+          return true;
+        };
+        ok = ok && wait_k(0);
+        for (int t = 0; t < 2 && ok; ++t)
+          if (sp[t].sees(key0(0), a.sinks)) ok = issue_s(t, 0);
+        if (ok) umma_commit(&k_empty[0]);
+        for (int n = 0; n < n_all && ok; ++n) {
+          const bool more = n + 1 < n_all;
+          if (more) ok = wait_k(n + 1);
+          if (!C::kAlias && more) {
+            for (int t = 0; t < 2 && ok; ++t)
+              if (sp[t].sees(key0(n + 1), a.sinks)) ok = issue_s(t, n + 1);
+            if (ok) umma_commit(&k_empty[(n + 1) % C::kRing]);
+          }
+          if (ok) ok = mbar_wait(&v_full[n % C::kRing], (n / C::kRing) & 1, status, kStatusTimeoutFull);
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (sp[t].sees(key0(n), a.sinks)) ok = issue_pv(t, n);
+            if (C::kAlias && more && ok && sp[t].sees(key0(n + 1), a.sinks)) ok = issue_s(t, n + 1);
+          }
+          if (ok) {
+            umma_commit(&v_empty[n % C::kRing]);
+            if (C::kAlias && more) umma_commit(&k_empty[(n + 1) % C::kRing]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+    const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
+    const Span me = sp[t];
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tS = tmem + C::kColS + t * 128 + lanes, tP = tmem + C::kColP + t * C::kStepP + lanes;
+    const uint32_t tO = tmem + C::kColO + t * D + lanes;
+    const float c = a.scale * 1.4426950408889634f;
+    const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
+    const int row_hi = min(kl - 1, p + a.right), row_lo = p - a.left;
+    float m = -INFINITY, l = 0.f;
+    int cnt = 0;
+    bool ok = true;
+    for (int n = 0; n < n_all && ok; ++n) {
+      const int k0 = key0(n);
+      if (!me.sees(k0, a.sinks)) continue;
+      ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
+      if (!ok) break;
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[32];
+        tmem_ld32(tS + 32 * i, w);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[32 * i + j] = __uint_as_float(w[j]);
+      }
+      tmem_wait_ld();
+      if (!C::kAlias) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+      }
+      if (!me.whole(k0, a.sinks)) {
+        // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
+        const int x1 = row_hi - k0, x0 = row_lo - k0, x2 = a.sinks - k0;
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (i > x1 || (i < x0 && i >= x2)) s[i] = -INFINITY;
+      }
+      float m8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[120 + i]);
+#pragma unroll
+      for (int i = 8; i < 120; i += 16)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
+      const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
+      // P of the last tile has been read and O_t is complete (with P over S, S_t of this
+      // tile was issued after that product)
+      if (!C::kAlias && cnt > 0) {
+        ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool raise = cnt == 0 || (mt - m) * c > kRaise;
+      if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
+        const float alpha = raise ? ex2_approx((m - mt) * c) : 1.f;
+#pragma unroll
+        for (int i = 0; i < D; i += 32) {
+          uint32_t w[32];
+          tmem_ld32(tO + i, w);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+          tmem_st32(tO + i, w);
+        }
+        tmem_wait_st();
+        l *= alpha;
+      }
+      if (raise) m = mt;
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 x = __ffma2_rn(make_float2(s[64 * hf + 2 * i], s[64 * hf + 2 * i + 1]), make_float2(c, c),
+                                      make_float2(-mc, -mc));
+          const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+          pk[i] = pack2<BF16>(e.x, e.y);
+        }
+        tmem_st32(tP + 32 * hf, pk);
+      }
+      const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+      l += s2.x + s2.y;
+      tmem_wait_st();
+      // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
+      if (k0 + kKT - 1 > hi || (k0 < lo && k0 + kKT > a.sinks)) {
+        ok = mbar_wait_warp(&v_full[n % C::kRing], (n / C::kRing) & 1, status, kStatusTimeoutFull);
+        if (!ok) break;
+        const int key = k0 + r;
+        if (key > hi || (key < lo && key >= a.sinks)) {
+          uint4* row = reinterpret_cast<uint4*>(sV + n % C::kRing * C::kTile + r * 128);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) row[(i >> 3) * 1024 + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
+      ++cnt;
+    }
+    if (ok && cnt > 0) {
+      ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+      tc_fence_after();
+    }
+    // O / l, 64 columns at a time through this warp's part of its (now idle) Q tile. A row
+    // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
+    // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
+    if (__all_sync(0xffffffffu, ok) && me.n > 0) {
+      const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
+      uint8_t* stg = sQ + t * C::kTile + q * 4096;
+      const int rows = me.n * g;
+#pragma unroll 1
+      for (int ch = 0; ch < D / 64; ++ch) {
+        uint32_t w[64];
+        if (cnt > 0) {
+          uint32_t w0_[32], w1_[32];
+          tmem_ld32(tO + 64 * ch, w0_);
+          tmem_ld32(tO + 64 * ch + 32, w1_);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            w[i] = w0_[i];
+            w[32 + i] = w1_[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) w[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint4 u;
+          uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            uw[j] = pack2<BF16>(__uint_as_float(w[8 * i + 2 * j]) * inv, __uint_as_float(w[8 * i + 2 * j + 1]) * inv);
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((i ^ (lane & 7)) << 4)) = u;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = 4 * k + (lane >> 3), ci = lane & 7, rr = q * 32 + row;
+          const uint4 u = *reinterpret_cast<const uint4*>(stg + row * 128 + ((ci ^ (row & 7)) << 4));
+          const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + rr / g) * a.os.tok +
+                              static_cast<int64_t>(h0 + rr % g) * a.os.head + ch * 64 + ci * 8;
+          if (rr < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) = u;
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// 4-D tensor map (head_dim, heads, tokens, sequences) of a 16-bit tensor: boxes of 64 dims x
+// box_heads x box_tokens, 128B swizzle, zero fill out of range.
+int map_4d(CUtensorMap* m, const void* p, const Strides& st, int bf16, int D, int heads, int len, int nseq, int box_heads,
+           int box_tokens) {
+  const int64_t dims[4] = {D, heads, len, nseq};
+  const int64_t strides[3] = {st.head * 2, st.tok * 2, st.seq * 2};
+  const int box[4] = {64, box_heads, box_tokens, 1};
+  return make_tmap_4d(m, p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, strides, box);
+}
+
+template <int D, bool BF16>
+int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
+  using C = WinCfg<D>;
+  // query heads side by side in a tile: the largest divisor of the sharing that fits
+  const int share = a.heads / a.kv_heads;
+  int g = 1;
+  for (int d = 2; d <= 32 && d <= share; ++d)
+    if (share % d == 0) g = d;
+  const int tokens = 128 / g;
+  CUtensorMap tq, tk, tv;
+  if (map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
+      map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT) ||
+      map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT))
+    return -2;
+  static std::atomic<uint64_t> attr_set{0};  // one bit per device; first calls may race
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((attr_set.load() >> (dev & 63)) & 1)) {
+    if (cudaFuncSetAttribute(k_attn_tiles<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+      return -3;
+    // the register split waits for registers that the launch must have
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, k_attn_tiles<D, BF16>) != cudaSuccess ||
+        fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsSoft)
+      return -5;
+    attr_set.fetch_or(uint64_t(1) << (dev & 63));
+  }
+  const int tiles = (a.q_len + 2 * tokens - 1) / (2 * tokens);
+  const int64_t ctas = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
+  if (ctas > 0x7fffffff) return -1;
+  k_attn_tiles<D, BF16><<<static_cast<unsigned>(ctas), kThreads, C::kSmem, s>>>(tq, tk, tv, a, g, tokens, tiles, status);
+  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+}
+
 }  // namespace
 
 int attention_window(const AttnWindow& a, int* status, cudaStream_t s) {
-  (void)status;
+  if (a.q_len > 1 && a.k_len > 0) {
+    if (a.bf16) return a.head_dim == 64 ? launch_tiles<64, true>(a, status, s) : launch_tiles<128, true>(a, status, s);
+    return a.head_dim == 64 ? launch_tiles<64, false>(a, status, s) : launch_tiles<128, false>(a, status, s);
+  }
   const long rows = static_cast<long>(a.nseq) * a.heads * a.q_len;
   const unsigned grid = static_cast<unsigned>((rows + 7) / 8);
   if (a.bf16) {

@@ -1254,6 +1254,27 @@ int make_tmap_2d_typed(CUtensorMap* map, const void* ptr, CUtensorMapDataType dt
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
+int make_tmap_4d(CUtensorMap* map, const void* ptr, CUtensorMapDataType dtype, const int64_t* dims,
+                 const int64_t* strides, const int* box) {
+  PFN_tmapEncodeTiled enc = tmap_encoder();
+  if (!enc) return -1;
+  if (reinterpret_cast<uintptr_t>(ptr) & 15) return -2;
+  cuuint64_t d[4], st[3];
+  cuuint32_t bx[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) {
+    if (dims[i] < 1 || box[i] < 1 || box[i] > 256) return -2;
+    d[i] = static_cast<cuuint64_t>(dims[i]);
+    bx[i] = static_cast<cuuint32_t>(box[i]);
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (strides[i] <= 0 || strides[i] % 16) return -2;
+    st[i] = static_cast<cuuint64_t>(strides[i]);
+  }
+  CUresult r = enc(map, dtype, 4, const_cast<void*>(ptr), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
 // 4-D f16 tensor map over an NHWC tensor [B][H][W][C] (row pitch C), box =
 // 64 channels x bw x bh x 1, 128B swizzle, zero fill out of range (conv padding).
 int make_tmap_nhwc(CUtensorMap* map, const void* ptr, int B, int H, int W, int C, int bw, int bh) {

@@ -14,6 +14,10 @@ int make_tmap_2d(CUtensorMap* map, const void* ptr, int rows, int cols, int ld, 
 int make_tmap_nhwc(CUtensorMap* map, const void* ptr, int B, int H, int W, int C, int bw, int bh);
 int make_tmap_2d_typed(CUtensorMap* map, const void* ptr, CUtensorMapDataType dtype, int elem_bytes, int rows,
                        int cols, int ld, int box_cols, int box_rows, CUtensorMapSwizzle swz);
+// 4-D map of a 16-bit type: dims and box innermost first, byte strides of dims 1..3, 128B
+// swizzle, zero fill out of range.
+int make_tmap_4d(CUtensorMap* map, const void* ptr, CUtensorMapDataType dtype, const int64_t* dims,
+                 const int64_t* strides, const int* box);
 int make_tmap_nhwc_planes(CUtensorMap* map, const void* ptr, int B, int H, int W, int C, int bw, int bh);
 int gemm_launch(int bn, const CUtensorMap& ta, const CUtensorMap& tb, const GemmGeom& g, const EpiArgs& e,
                 int* status, cudaStream_t stream, int max_ctas);
