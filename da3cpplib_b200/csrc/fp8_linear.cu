@@ -531,7 +531,7 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
     // the register split waits for registers that the launch must have
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, k_fp8_gemm<CG>) != cudaSuccess ||
-        fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsEpi)
+        fa.numRegs * kThreads < 128 * kRegsCtl + 512 * kRegsEpi)
       return -5;
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
