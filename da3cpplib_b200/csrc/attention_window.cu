@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) k_attn_window(const AttnWindow a) {
 
 
 // ------------------------------------------------------------------ many queries
-// Two tiles of 128 query rows a CTA (one CTA per SM, 20 warps), key tiles of 128 shared by
+// Two tiles of 128 query rows a CTA (one CTA per SM, 12 warps), key tiles of 128 shared by
 // both. A query row is one (token, head): g query heads that share a key head lie side by
 // side, 128 / g tokens a tile, so that shared heads read their keys once and a tile spans
 // few positions (a window's ends are masked work).
@@ -72,12 +72,11 @@ __global__ void __launch_bounds__(256) k_attn_window(const AttnWindow a) {
 //              ring of its own ([128 keys][64 dims] boxes, 128B swizzle);
 //   warp 1     one thread issues S_t = Q_t K^T (M = N = 128) and O_t += P_t V (P_t from
 //              tensor memory; V is read as it lies, its dims contiguous: an MN-major operand);
-//   warps 4-19 softmax, eight a query tile: thread = row (its TMEM lane) and one half of the
-//              tile's 128 keys; its 64 scores in registers, one pass; P back to tensor
-//              memory. The two threads of a row exchange their maxima through shared memory.
-//              Four softmax warps an SM sub-partition hide each other's latencies: with one
-//              thread a row (two warps a sub-partition) full attention at head_dim 64 ran at
-//              590 TFLOP/s, its chain of TMEM loads, maxima and exponentials exposed.
+//   warps 4-7  softmax of query tile 0, warps 8-11 of tile 1: thread = row (its TMEM lane),
+//              the row's 128 scores in registers, one pass; P back to tensor memory. Two
+//              threads a row (half the keys each, maxima exchanged through shared memory)
+//              took longer: 2300 cycles a tile against 1500, as the four warps of an SM
+//              sub-partition then take their exponentials at the same time.
 // Tensor memory (512 columns): head_dim 64: S_t 128, P_t 64, O_t 64 columns each, so S_t of
 // the next key tile is issued as soon as the scores are in registers, while their
 // exponentials are taken. head_dim 128: O_t takes 128 columns and P_t lies over S_t, so
@@ -89,19 +88,18 @@ __global__ void __launch_bounds__(256) k_attn_window(const AttnWindow a) {
 
 constexpr int kKT = 128;                // keys per tile
 constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the row's maximum
-constexpr int kThreads = 640;
-// Launched at 96 registers a thread (61 440 in all): the first warpgroup gives back down to
-// 40, the softmax's four warpgroups take 104.
-constexpr int kRegsLaunch = 96, kRegsCtl = 40, kRegsSoft = 104;
-static_assert(128 * kRegsCtl + 512 * kRegsSoft <= kThreads * kRegsLaunch, "register split exceeds the launch");
+constexpr int kThreads = 384;
+// Launched at 168 registers a thread (64 512 in all): the first warpgroup gives back down to
+// 56, the softmax's two warpgroups take 224.
+constexpr int kRegsLaunch = 168, kRegsCtl = 56, kRegsSoft = 224;
+static_assert(128 * kRegsCtl + 256 * kRegsSoft <= kThreads * kRegsLaunch, "register split exceeds the launch");
 
 template <int D>
 struct WinCfg {
   static constexpr bool kAlias = D == 128;      // P over S
   static constexpr int kTile = 128 * D * 2;     // bytes of a Q, K or V tile
   static constexpr int kRing = D == 64 ? 4 : 2; // K tiles and V tiles in flight
-  static constexpr int kExchange = 2 * 2 * 2 * 128 * 4;  // row values [tile][parity][half][row]
-  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kRing * kTile + kExchange + 256;
+  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kRing * kTile + 256;
   static constexpr uint32_t kColS = 0, kColP = kAlias ? 0 : 256, kStepP = kAlias ? 128 : 64;
   static constexpr uint32_t kColO = kAlias ? 256 : 384;
 };
@@ -198,18 +196,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sQ = smem;                       // [2] tiles
   uint8_t* sK = sQ + 2 * C::kTile;          // [kRing]
   uint8_t* sV = sK + C::kRing * C::kTile;   // [kRing]
-  float* sX = reinterpret_cast<float*>(sV + C::kRing * C::kTile);
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sX + 2 * 2 * 2 * 128);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + C::kRing * C::kTile);
   uint64_t* k_full = q_full + 1;            // [kRing] each
   uint64_t* k_empty = k_full + C::kRing;
   uint64_t* v_full = k_empty + C::kRing;
   uint64_t* v_empty = v_full + C::kRing;
   uint64_t* s_full = v_empty + C::kRing;    // [2] S_t complete
-  uint64_t* s_free = s_full + 2;            // [2] S_t in registers (8 warps)
-  uint64_t* p_ready = s_free + 2;           // [2] P_t written, O_t rescaled, V rows zeroed (8 warps)
+  uint64_t* s_free = s_full + 2;            // [2] S_t in registers (4 warps)
+  uint64_t* p_ready = s_free + 2;           // [2] P_t written, O_t rescaled, V rows zeroed (4 warps)
   uint64_t* pv_done = p_ready + 2;          // [2] P_t V complete
-  uint64_t* swapped = pv_done + 2;          // [2] the halves' row values of tile t in sX (8 warps)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(swapped + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile2 = static_cast<int>(blockIdx.x) % tiles;
@@ -237,10 +233,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_free[t], 8);
-      mbar_init(&p_ready[t], 8);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&p_ready[t], 4);
       mbar_init(&pv_done[t], 1);
-      mbar_init(&swapped[t], 8);
     }
     fence_mbar_init();
     prefetch_tmap(&tmQ);
@@ -357,41 +352,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
-    const int t = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, q = warp & 3, r = q * 32 + lane;
-    const Span me = sp[t];
+    const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
+    const Span me = t == 0 ? sp[0] : sp[1];  // (an indexed array would live in local memory)
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tS = tmem + C::kColS + t * 128 + 64 * half + lanes;
-    const uint32_t tP = tmem + C::kColP + t * C::kStepP + 32 * half + lanes;
-    const uint32_t tO = tmem + C::kColO + t * D + half * (D / 2) + lanes;  // this half's columns of O
+    const uint32_t tS = tmem + C::kColS + t * 128 + lanes, tP = tmem + C::kColP + t * C::kStepP + lanes;
+    const uint32_t tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
     const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
     const int row_hi = min(kl - 1, p + a.right), row_lo = p - a.left;
     float m = -INFINITY, l = 0.f;
     int cnt = 0;
-    uint32_t swaps = 0;
     bool ok = true;
-    // the other half's value of this row; false if the wait ran out
-    auto swap = [&](float mine, float* theirs) -> bool {
-      float* x = sX + (t * 2 + (swaps & 1)) * 256 + r;
-      x[half * 128] = mine;
-      tc_fence_before();  // this warp's loads of S_t come before the other half's P_t
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&swapped[t]);
-      if (!mbar_wait_warp(&swapped[t], swaps & 1, status, kStatusTimeoutAccum)) return false;
-      tc_fence_after();
-      *theirs = x[(half ^ 1) * 128];
-      ++swaps;
-      return true;
-    };
-    for (int n = 0; n < n_all; ++n) {
+    for (int n = 0; n < n_all && ok; ++n) {
       const int k0 = key0(n);
       if (!me.sees(k0, a.sinks)) continue;
       ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
-      float s[64];
+      float s[128];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         uint32_t w[32];
         tmem_ld32(tS + 32 * i, w);
 #pragma unroll
@@ -404,35 +384,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&s_free[t]);
       }
       if (!me.whole(k0, a.sinks)) {
-        // visible columns of this row: [x0, x1] and [0, x2) of its half tile, up to x1
-        const int kh = k0 + 64 * half, x1 = row_hi - kh, x0 = row_lo - kh, x2 = a.sinks - kh;
+        // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
+        const int x1 = row_hi - k0, x0 = row_lo - k0, x2 = a.sinks - k0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < 128; ++i)
           if (i > x1 || (i < x0 && i >= x2)) s[i] = -INFINITY;
       }
       float m8[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[56 + i]);
+      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[120 + i]);
 #pragma unroll
-      for (int i = 8; i < 56; i += 16)
+      for (int i = 8; i < 120; i += 16)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
-      float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]), other;
-      ok = swap(mt, &other);
-      if (!ok) break;
-      mt = fmaxf(mt, other);
+      const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
       const bool raise = cnt == 0 || (mt - m) * c > kRaise;
       const float alpha = raise ? ex2((m - mt) * c) : 1.f;
       if (raise) m = mt;
       const float mc = m == -INFINITY ? 0.f : m * c;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      uint32_t pk[32];
+      uint32_t pk[2][32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < 64; ++i) {
         const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(-mc, -mc));
         const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
         sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-        pk[i] = pack2<BF16>(e.x, e.y);
+        pk[i >> 5][i & 31] = pack2<BF16>(e.x, e.y);
       }
       const float2 s2 = __fadd2_rn(sum[0], sum[1]);
       // P of the last tile has been read and O_t is complete (with P over S, S_t of this
@@ -444,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
-        for (int i = 0; i < D / 2; i += 16) {
+        for (int i = 0; i < D; i += 16) {
           uint32_t w[16];
           tmem_ld16(tO + i, w);
           tmem_wait_ld();
@@ -455,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= alpha;
       }
       l += s2.x + s2.y;
-      tmem_st32(tP, pk);
+      tmem_st32(tP, pk[0]);
+      tmem_st32(tP + 32, pk[1]);
       tmem_wait_st();
       // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
       if (k0 + kKT - 1 > hi || (k0 < lo && k0 + kKT > a.sinks)) {
@@ -465,10 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (key > hi || (key < lo && key >= a.sinks)) {
           uint4* row = reinterpret_cast<uint4*>(sV + n % C::kRing * C::kTile + r * 128);
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const int j = half * (D / 16) + i;
-            row[(j >> 3) * 1024 + (j & 7)] = make_uint4(0u, 0u, 0u, 0u);
-          }
+          for (int i = 0; i < D / 8; ++i) row[(i >> 3) * 1024 + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_proxy_async_smem();
       }
@@ -481,48 +456,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
       tc_fence_after();
     }
-    // O / l of this half's columns, through this warp's part of its (now idle) Q tile. A row
+    // O / l, 64 columns at a time through this warp's part of its (now idle) Q tile. A row
     // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
     // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
-    float l2 = 0.f;
-    if (ok && me.n > 0) ok = swap(l, &l2);
-    if (ok && me.n > 0) {
-      l += l2;
+    if (__all_sync(0xffffffffu, ok) && me.n > 0) {
       const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
-      constexpr int kChunks = D / 16;  // 16-byte chunks of a row's half
-      uint8_t* stg = sQ + t * C::kTile + (half * 4 + q) * (32 * kChunks * 16);
+      uint8_t* stg = sQ + t * C::kTile + q * 4096;
       const int rows = me.n * g;
-      // rows of 64 bytes share a 128-byte line two by two
-      auto at = [&](int row, int ch) { return stg + row * (kChunks * 16) + ((ch ^ (D == 64 ? (row >> 1) & 3 : row & 7)) << 4); };
-#pragma unroll
-      for (int i = 0; i < kChunks; i += 2) {
-        uint32_t w[16];
+#pragma unroll 1
+      for (int ch = 0; ch < D / 64; ++ch) {
+        uint32_t w[64];
         if (cnt > 0) {
-          tmem_ld16(tO + 8 * i, w);
+          uint32_t w0_[32], w1_[32];
+          tmem_ld32(tO + 64 * ch, w0_);
+          tmem_ld32(tO + 64 * ch + 32, w1_);
           tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            w[i] = w0_[i];
+            w[32 + i] = w1_[i];
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = 0u;
+          for (int i = 0; i < 64; ++i) w[i] = 0u;
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int i = 0; i < 8; ++i) {
           uint4 u;
           uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            uw[j] = pack2<BF16>(__uint_as_float(w[8 * k + 2 * j]) * inv, __uint_as_float(w[8 * k + 2 * j + 1]) * inv);
-          *reinterpret_cast<uint4*>(at(lane, i + k)) = u;
+            uw[j] = pack2<BF16>(__uint_as_float(w[8 * i + 2 * j]) * inv, __uint_as_float(w[8 * i + 2 * j + 1]) * inv);
+          *reinterpret_cast<uint4*>(stg + lane * 128 + ((i ^ (lane & 7)) << 4)) = u;
         }
-      }
-      __syncwarp();
-      constexpr int kRows = 32 / kChunks;  // rows a store instruction covers
+        __syncwarp();
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-        const int row = kRows * k + lane / kChunks, ci = lane % kChunks, rr = q * 32 + row;
-        const uint4 u = *reinterpret_cast<const uint4*>(at(row, ci));
-        const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + rr / g) * a.os.tok +
-                            static_cast<int64_t>(h0 + rr % g) * a.os.head + half * (D / 2) + ci * 8;
-        if (rr < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) = u;
+        for (int k = 0; k < 8; ++k) {
+          const int row = 4 * k + (lane >> 3), ci = lane & 7, rr = q * 32 + row;
+          const uint4 u = *reinterpret_cast<const uint4*>(stg + row * 128 + ((ci ^ (row & 7)) << 4));
+          const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + rr / g) * a.os.tok +
+                              static_cast<int64_t>(h0 + rr % g) * a.os.head + ch * 64 + ci * 8;
+          if (rr < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) = u;
+        }
+        __syncwarp();
       }
     }
   }
@@ -567,7 +543,7 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
     // the register split waits for registers that the launch must have
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, k_attn_tiles<D, BF16>) != cudaSuccess ||
-        fa.numRegs * kThreads < 128 * kRegsCtl + 512 * kRegsSoft)
+        fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsSoft)
       return -5;
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
