@@ -4,6 +4,7 @@
 // (the queries are the last ones of the keys) and sees the keys j < kl with
 // j <= p + right and (j >= p - left or j < sinks). o = sum_j softmax_j(scale q.k_j) v_j; a
 // query that sees nothing gets zeros, rows from ql on are not written.
+#include <algorithm>
 #include <atomic>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -20,48 +21,6 @@
 namespace da3b {
 
 namespace {
-
-// Reference form: one warp per (query, head), one key at a time, D / 32 dims a lane.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_attn_window(const AttnWindow a) {
-  constexpr int E = D / 32;
-  const long w = static_cast<long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= static_cast<long>(a.nseq) * a.heads * a.q_len) return;
-  const int i = static_cast<int>(w % a.q_len), h = static_cast<int>(w / a.q_len % a.heads);
-  const int b = static_cast<int>(w / a.q_len / a.heads);
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-  const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
-  if (i >= ql) return;
-  const int hk = h / (a.heads / a.kv_heads), p = kl - ql + i;
-  const T* q = static_cast<const T*>(a.q) + b * a.qs.seq + i * a.qs.tok + h * a.qs.head + lane * E;
-  const T* k = static_cast<const T*>(a.k) + b * a.ks.seq + hk * a.ks.head + lane * E;
-  const T* v = static_cast<const T*>(a.v) + b * a.vs.seq + hk * a.vs.head + lane * E;
-  float o[E] = {}, l = 0.f, m = -INFINITY;
-  const int hi = min(kl - 1, p + a.right), lo = max(p - a.left, 0);
-  const float c = a.scale * 1.4426950408889634f;
-  for (int j = 0; j <= hi; ++j) {
-    if (j < lo && j >= a.sinks) {
-      j = lo - 1;
-      continue;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(static_cast<float>(q[e]), static_cast<float>(k[j * a.ks.tok + e]), s);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f((m - base) * c), pr = exp2f((s - base) * c);
-    m = mn;
-    l = l * alpha + pr;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + pr * static_cast<float>(v[j * a.vs.tok + e]);
-  }
-  T* out = static_cast<T*>(a.out) + b * a.os.seq + i * a.os.tok + h * a.os.head + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[e] = static_cast<T>(l > 0.f ? o[e] / l : (l == 0.f ? 0.f : l));
-}
-
 
 // ------------------------------------------------------------------ many queries
 // Two tiles of 128 query rows a CTA (one CTA per SM, 12 warps), key tiles of 128 shared by
@@ -554,23 +513,371 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? 0 : -4;
 }
 
+// ------------------------------------------------------------------ few queries
+// At most 16 query rows ((token, head) pairs of a key head): every visible K and V byte is
+// read once and that bounds the kernel. A CTA takes one (sequence, key head), or a share of
+// its keys when there are too few of those to fill the SMs: the CTAs of a cluster then join
+// their sums through distributed shared memory. Key tiles of 64 arrive by TMA in a ring; each
+// of four warps takes 16 keys of a tile with m16n8k16 products (the rows padded to 16; the
+// tensor work is far below the memory's time, so the small warp-level form is enough) and
+// keeps its own running maximum, sum and output, joined at the end.
+constexpr int kFewRows = 16, kFewKeys = 64, kFewWarps = 4, kFewThreads = 32 * (kFewWarps + 1);
+
+template <int D>
+struct FewCfg {
+  static constexpr int kTile = kFewKeys * D * 2;           // bytes of a K or V tile
+  static constexpr int kStages = D == 64 ? 6 : 3;          // about 96 KB in flight, two CTAs an SM
+  static constexpr int kPartFloats = kFewRows * (D + 2);   // O rows, then maxima and sums
+  static constexpr int kSmem = 1024 + kStages * 2 * kTile + 128;
+  static_assert((kFewWarps + 1) * kPartFloats * 4 <= kStages * 2 * kTile, "partial sums fit the ring");
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kFewThreads, 2)
+    k_attn_few(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+               const __grid_constant__ AttnWindow a, int nsplit, int* status) {
+  using C = FewCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * 2 * C::kTile);
+  uint64_t* empty = full + C::kStages;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
+  const int hk = item % a.kv_heads, b = item / a.kv_heads;
+  const int share = a.heads / a.kv_heads;
+  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+  const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
+  const int rows = ql * share;
+  // keys some row sees: [lo, hi] and [0, s0); tiles of the latter first
+  const int hi = min(kl - 1, kl - 1 + a.right), lo = max(0, kl - ql - a.left);
+  const int s0 = min(a.sinks, lo);
+  const int n_sink = (s0 + kFewKeys - 1) / kFewKeys;
+  const int n_all = rows == 0 || hi < 0 ? 0 : n_sink + (hi - lo + kFewKeys) / kFewKeys;
+  const int n_begin = static_cast<int>(static_cast<int64_t>(split) * n_all / nsplit);
+  const int n_end = static_cast<int>(static_cast<int64_t>(split + 1) * n_all / nsplit);
+  auto key0 = [&](int n) { return n < n_sink ? n * kFewKeys : lo + (n - n_sink) * kFewKeys; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kFewWarps);
+    }
+    fence_mbar_init();
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  __syncthreads();
+
+  float o[D / 8][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+  bool ok = true;
+
+  if (warp == kFewWarps) {
+    if (lane == 0) {
+      for (int n = n_begin; n < n_end; ++n) {
+        const int it = n - n_begin, st = it % C::kStages;
+        if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1u, status, kStatusTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
+        uint8_t* k = smem + st * 2 * C::kTile;
+        for (int c = 0; c < D / 64; ++c) tma_load_4d(k + c * 8192, &tmK, &full[st], c * 64, hk, key0(n), b);
+        for (int c = 0; c < D / 64; ++c) tma_load_4d(k + C::kTile + c * 8192, &tmV, &full[st], c * 64, hk, key0(n), b);
+      }
+    }
+    __syncwarp();
+  } else {
+    const float c = a.scale * 1.4426950408889634f;
+    // Q fragments: rows lane / 4 and + 8, dims 16 i + 2 (lane % 4) and + 8
+    uint32_t q[D / 16][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = lane / 4 + 8 * j;
+      const uint16_t* row = static_cast<const uint16_t*>(a.q) + b * a.qs.seq + static_cast<int64_t>(r / share) * a.qs.tok +
+                            static_cast<int64_t>(hk * share + r % share) * a.qs.head;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          q[i][j + 2 * h] = r < rows ? *reinterpret_cast<const uint32_t*>(row + 16 * i + 8 * h + 2 * (lane % 4)) : 0u;
+    }
+    const int p0 = kl - ql + (lane / 4) / share, p1 = kl - ql + (lane / 4 + 8) / share;  // the rows' positions
+    const int row_hi[2] = {min(kl - 1, p0 + a.right), min(kl - 1, p1 + a.right)}, row_lo[2] = {p0 - a.left, p1 - a.left};
+    for (int n = n_begin; n < n_end; ++n) {
+      const int it = n - n_begin, st = it % C::kStages, k0 = key0(n);
+      ok = mbar_wait_warp(&full[st], (it / C::kStages) & 1, status, kStatusTimeoutFull);
+      if (!ok) break;
+      const uint32_t sK = smem_u32(smem + st * 2 * C::kTile), sV = sK + C::kTile;
+      const int key_w = k0 + 16 * warp;  // this warp's first key
+      // S: 16 rows x 16 keys
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      {
+        const int r = 16 * warp + (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t kf[4];
+          ldmatrix4(sK + (i >> 2) * 8192 + r * 128 + (((2 * (i & 3) + ch) ^ (r & 7)) << 4), kf);
+          mma16816<BF16>(s[0], q[i], kf[0], kf[1]);
+          mma16816<BF16>(s[1], q[i], kf[2], kf[3]);
+        }
+      }
+      // keys that no row sees: masked, and their V rows zeroed (0 * NaN)
+      const bool sink_tile = n < n_sink;
+      const int key_end = sink_tile ? min(s0, hi + 1) : hi + 1;
+      if (key_w + 16 > key_end) {
+        const int dead = max(0, key_end - key_w);  // first dead key of the warp's 16
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int chunk = lane + 32 * i, r = chunk / (D / 8), cc = chunk % (D / 8);
+          if (r >= dead)
+            *reinterpret_cast<uint4*>(smem + st * 2 * C::kTile + C::kTile + (cc >> 3) * 8192 + (16 * warp + r) * 128 +
+                                      (cc & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      // mask by row where the tile is not seen whole by every row
+      if (sink_tile || key_w + 15 > kl - ql + a.right || key_w + 16 > key_end || key_w < kl - 1 - a.left) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key_w + 8 * j + 2 * (lane % 4) + (e & 1), rr = e >> 1;
+            const bool sees = key < key_end && key <= row_hi[rr] && (key >= row_lo[rr] || key < a.sinks);
+            if (!sees) s[j][e] = -INFINITY;
+          }
+      }
+      float mt[2];
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        mt[rr] = fmaxf(fmaxf(s[0][2 * rr], s[0][2 * rr + 1]), fmaxf(s[1][2 * rr], s[1][2 * rr + 1]));
+        mt[rr] = fmaxf(mt[rr], __shfl_xor_sync(0xffffffffu, mt[rr], 1));
+        mt[rr] = fmaxf(mt[rr], __shfl_xor_sync(0xffffffffu, mt[rr], 2));
+      }
+      if (__any_sync(0xffffffffu, mt[0] > m[0] || mt[1] > m[1])) {
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+          const float mn = fmaxf(m[rr], mt[rr]);
+          const float alpha = m[rr] == mn ? 1.f : ex2((m[rr] - mn) * c);
+          m[rr] = mn;
+          l[rr] *= alpha;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][2 * rr] *= alpha;
+            o[i][2 * rr + 1] *= alpha;
+          }
+        }
+      }
+      uint32_t pf[4];
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        const float mc = m[rr] == -INFINITY ? 0.f : m[rr] * c;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float e0 = ex2(fmaf(s[j][2 * rr], c, -mc)), e1 = ex2(fmaf(s[j][2 * rr + 1], c, -mc));
+          l[rr] += e0 + e1;
+          pf[rr + 2 * j] = pack2<BF16>(e0, e1);
+        }
+      }
+      {
+        const int r = 16 * warp + (lane & 15), ch = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t vf[4];
+          ldmatrix4_trans(sV + (i >> 2) * 8192 + r * 128 + (((2 * (i & 3) + ch) ^ (r & 7)) << 4), vf);
+          mma16816<BF16>(o[2 * i], pf, vf[0], vf[1]);
+          mma16816<BF16>(o[2 * i + 1], pf, vf[2], vf[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
+#pragma unroll
+    for (int rr = 0; rr < 2; ++rr) {
+      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
+      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
+    }
+  }
+
+  // Join the warps: each leaves O, maxima and sums in the ring (every tile has been read).
+  // part[w]: [16][D], then [16] maxima, [16] sums; part[kFewWarps] is the CTA's.
+  const int bad = __syncthreads_or(!ok);
+  float* part = reinterpret_cast<float*>(smem);
+  if (warp < kFewWarps) {
+    float* w = part + warp * C::kPartFloats;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr)
+        *reinterpret_cast<float2*>(w + (lane / 4 + 8 * rr) * D + 8 * i + 2 * (lane % 4)) =
+            make_float2(o[i][2 * rr], o[i][2 * rr + 1]);
+    if (lane % 4 == 0) {
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {
+        w[kFewRows * D + lane / 4 + 8 * rr] = m[rr];
+        w[kFewRows * D + kFewRows + lane / 4 + 8 * rr] = l[rr];
+      }
+    }
+  }
+  __syncthreads();
+  const float c = a.scale * 1.4426950408889634f;
+  // weights of n partial sums with maxima m_i, in order: 2^((m_i - max) c), 0 for one that
+  // saw no key; max over finite scores only where there is one
+  auto weight = [&](float mi, float mx) { return mi == -INFINITY ? 0.f : ex2((mi - mx) * c); };
+  float* mine = part + kFewWarps * C::kPartFloats;
+  for (int e = threadIdx.x; e < kFewRows * D / 2; e += kFewThreads) {
+    const int r = e / (D / 2), d = e % (D / 2) * 2;
+    float mx = -INFINITY, sum = 0.f;
+    float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, part[w * C::kPartFloats + kFewRows * D + r]);
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float* pw = part + w * C::kPartFloats;
+      const float lw = pw[kFewRows * D + kFewRows + r];
+      // a NaN sum (NaN scores only: the maximum passed them by) is kept
+      const float f = lw == lw ? weight(pw[kFewRows * D + r], mx) : 1.f;
+      sum += f * lw;
+      const float2 x = *reinterpret_cast<const float2*>(pw + r * D + d);
+      v.x += f * x.x;
+      v.y += f * x.y;
+    }
+    *reinterpret_cast<float2*>(mine + r * D + d) = v;
+    if (d == 0) {
+      mine[kFewRows * D + r] = mx;
+      mine[kFewRows * D + kFewRows + r] = sum;
+    }
+  }
+  if (nsplit > 1) cluster_sync();
+  else __syncthreads();
+  // Join the CTAs of the cluster in rank order; each writes its share of the elements.
+  if (!bad) {
+    const uint32_t base = smem_u32(mine);
+    const int pairs = rows * D / 2;
+    for (int e = split * kFewThreads + static_cast<int>(threadIdx.x); e < pairs; e += nsplit * kFewThreads) {
+      const int r = e / (D / 2), d = e % (D / 2) * 2;
+      float mx = -INFINITY, sum = 0.f;
+      float2 v = make_float2(0.f, 0.f);
+      if (nsplit == 1) {
+        mx = mine[kFewRows * D + r];
+        sum = mine[kFewRows * D + kFewRows + r];
+        v = *reinterpret_cast<const float2*>(mine + r * D + d);
+      } else {
+        for (int i = 0; i < nsplit; ++i) mx = fmaxf(mx, ld_dsmem_f1(mapa_shared(base + 4 * (kFewRows * D + r), i)));
+        for (int i = 0; i < nsplit; ++i) {
+          const float li = ld_dsmem_f1(mapa_shared(base + 4 * (kFewRows * D + kFewRows + r), i));
+          const float mi = ld_dsmem_f1(mapa_shared(base + 4 * (kFewRows * D + r), i));
+          const float2 x = ld_dsmem_f2(mapa_shared(base + 4 * (r * D + d), i));
+          const float f = li == li ? weight(mi, mx) : 1.f;
+          sum += f * li;
+          v.x += f * x.x;
+          v.y += f * x.y;
+        }
+      }
+      const float inv = mx == -INFINITY && sum == sum ? 0.f : 1.f / sum;  // no key seen: zeros
+      const int64_t off = b * a.os.seq + static_cast<int64_t>(r / share) * a.os.tok +
+                          static_cast<int64_t>(hk * share + r % share) * a.os.head + d;
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + off) = pack2<BF16>(v.x * inv, v.y * inv);
+    }
+  }
+  if (nsplit > 1) cluster_sync();  // no CTA leaves while another may still read its sums
+}
+
+template <int D, bool BF16>
+int launch_few(const AttnWindow& a, int* status, cudaStream_t s) {
+  using C = FewCfg<D>;
+  CUtensorMap tk, tv;
+  if (map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kFewKeys) ||
+      map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kFewKeys))
+    return -2;
+  static std::atomic<uint64_t> attr_set{0};  // one bit per device; first calls may race
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!((attr_set.load() >> (dev & 63)) & 1)) {
+    if (cudaFuncSetAttribute(k_attn_few<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+      return -3;
+    attr_set.fetch_or(uint64_t(1) << (dev & 63));
+  }
+  // Split the keys while the SMs' two slots each are not full and a share keeps four tiles
+  // (of the longest window that the sizes allow; lengths are on the device).
+  const int64_t items = static_cast<int64_t>(a.nseq) * a.kv_heads;
+  const int64_t window = static_cast<int64_t>(a.left) + a.q_len + a.sinks;
+  const int64_t tiles = (std::min<int64_t>(a.k_len, window) + kFewKeys - 1) / kFewKeys;
+  const int nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 296 / items, tiles / 4})));
+  if (items * nsplit > 0x7fffffff) return -1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(nsplit);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = nsplit > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_attn_few<D, BF16>, tk, tv, a, nsplit, status) == cudaSuccess ? 0 : -4;
+}
+
+// No keys at all (k_len 0; a tensor map cannot be empty): zeros in the rows that count.
+__global__ void k_attn_none(const AttnWindow a) {
+  const int64_t per_row = a.head_dim / 8;
+  const int64_t n = static_cast<int64_t>(a.nseq) * a.q_len * a.heads * per_row;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
+       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = e / per_row;
+    const int h = static_cast<int>(row % a.heads), i = static_cast<int>(row / a.heads % a.q_len);
+    const int b = static_cast<int>(row / a.heads / a.q_len);
+    if (a.q_lens && i >= a.q_lens[b]) continue;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + b * a.os.seq + i * a.os.tok + h * a.os.head +
+                              e % per_row * 8) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 }  // namespace
 
+template <int D, bool BF16>
+static int run(const AttnWindow& a, int* status, cudaStream_t s) {
+  // few rows for each key head: the memory-bound kernel (its tensor work is padded to 16
+  // rows, the tiled kernel's to 256)
+  if (static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads) <= kFewRows) return launch_few<D, BF16>(a, status, s);
+  return launch_tiles<D, BF16>(a, status, s);
+}
+
 int attention_window(const AttnWindow& a, int* status, cudaStream_t s) {
-  if (a.q_len > 1 && a.k_len > 0) {
-    if (a.bf16) return a.head_dim == 64 ? launch_tiles<64, true>(a, status, s) : launch_tiles<128, true>(a, status, s);
-    return a.head_dim == 64 ? launch_tiles<64, false>(a, status, s) : launch_tiles<128, false>(a, status, s);
+  if (a.k_len == 0) {
+    k_attn_none<<<256, 256, 0, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? 0 : -4;
   }
-  const long rows = static_cast<long>(a.nseq) * a.heads * a.q_len;
-  const unsigned grid = static_cast<unsigned>((rows + 7) / 8);
-  if (a.bf16) {
-    if (a.head_dim == 64) k_attn_window<__nv_bfloat16, 64><<<grid, 256, 0, s>>>(a);
-    else k_attn_window<__nv_bfloat16, 128><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (a.head_dim == 64) k_attn_window<__half, 64><<<grid, 256, 0, s>>>(a);
-    else k_attn_window<__half, 128><<<grid, 256, 0, s>>>(a);
-  }
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  if (a.bf16) return a.head_dim == 64 ? run<64, true>(a, status, s) : run<128, true>(a, status, s);
+  return a.head_dim == 64 ? run<64, false>(a, status, s) : run<128, false>(a, status, s);
 }
 
 }  // namespace da3b

@@ -265,6 +265,11 @@ __device__ __forceinline__ float4 ld_dsmem_f4(uint32_t caddr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ float ld_dsmem_f1(uint32_t caddr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(caddr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float2 ld_dsmem_f2(uint32_t caddr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(caddr) : "memory");
