@@ -49,8 +49,8 @@ constexpr int kKT = 128;                // keys per tile
 constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the row's maximum
 constexpr int kThreads = 384;
 // Launched at 168 registers a thread (64 512 in all): the first warpgroup gives back down to
-// 56, the softmax's two warpgroups take 224.
-constexpr int kRegsLaunch = 168, kRegsCtl = 56, kRegsSoft = 224;
+// 72, the softmax's two warpgroups take 216.
+constexpr int kRegsLaunch = 168, kRegsCtl = 72, kRegsSoft = 216;
 static_assert(128 * kRegsCtl + 256 * kRegsSoft <= kThreads * kRegsLaunch, "register split exceeds the launch");
 
 template <int D>
@@ -101,6 +101,17 @@ __device__ __forceinline__ float2 exp2_cubic(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
+// 32 columns of O; zeros where no product was made. Warp-collective.
+__device__ __forceinline__ void take_o(uint32_t taddr, bool any, uint32_t (&w)[32]) {
+  if (any) {
+    tmem_ld32(taddr, w);
+    tmem_wait_ld();
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) w[i] = 0u;
+  }
+}
+
 // Shared-memory descriptor of an MN-major operand tile in 128B-swizzled rows of 64 values:
 // 1024 bytes between groups of eight k rows, lbo bytes between 64-wide column chunks.
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
@@ -123,7 +134,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // What the rows of one query tile see: tokens [i0, i0 + n) of a sequence at positions from
-// p on.
+// p on. Keys are counted in columns (Columns below) once shifted.
 struct Span {
   int n;                 // tokens inside the sequence (0: the tile has no rows)
   int hi_min, hi_max;    // last visible key of its first and last row
@@ -136,19 +147,42 @@ struct Span {
     lo_min = max(0, p - left);
     lo_max = max(0, pl - left);
   }
-  __device__ bool sees(int k0, int sinks) const {  // some key of [k0, k0 + 128)
-    return n > 0 && k0 <= hi_max && (k0 + kKT > lo_min || k0 < sinks);
+  __device__ void shift(int by) {
+    hi_min += by;
+    hi_max += by;
+    lo_min += by;
+    lo_max += by;
   }
-  __device__ bool whole(int k0, int sinks) const {  // every row sees every key of the tile
-    return k0 + kKT - 1 <= hi_min && (k0 >= lo_max || k0 + kKT <= sinks);
+  __device__ bool sees(int v0, int sinks) const {  // some key of the tile at column v0
+    return n > 0 && v0 <= hi_max && (v0 + kKT > lo_min || v0 < sinks);
   }
+  __device__ bool whole(int v0, int sinks) const {  // every row sees every key of the tile
+    return v0 + kKT - 1 <= hi_min && (v0 >= lo_max || v0 + kKT <= sinks);
+  }
+};
+
+// The keys of a CTA as one run of columns: the sinks, up to a multiple of eight, then the
+// windows' keys from the oldest on, so that neither starts a tile of its own: four sinks and
+// a window of 1024 for 64 tokens are 9 tiles of 128 instead of 11. One tile may hold both; it
+// is loaded in boxes of eight rows.
+struct Columns {
+  int front;  // columns of the sinks (0: the columns are keys from `base` on)
+  int base;   // key of column `front`
+  __device__ Columns(int sinks, int lo) {
+    front = sinks > lo - kKT ? 0 : (sinks + 7) & ~7;
+    base = sinks > 0 && front == 0 ? 0 : lo;
+  }
+  __device__ int key(int v) const { return v < front ? v : base + v - front; }
+  __device__ int shift() const { return front - base; }  // key + shift = column
+  __device__ bool mixed(int v0) const { return v0 < front && front < v0 + kKT; }
 };
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnWindow a, int g, int tokens,
-                 int tiles, int* status) {
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK8,
+                 const __grid_constant__ CUtensorMap tmV8, const __grid_constant__ AttnWindow a, int g, int tokens,
+                 int tiles, int nsplit, int* status) {
   using C = WinCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -167,20 +201,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile2 = static_cast<int>(blockIdx.x) % tiles;
-  const int hg = static_cast<int>(blockIdx.x) / tiles % (a.heads / g);
-  const int b = static_cast<int>(blockIdx.x) / tiles / (a.heads / g);
+  // a cluster of nsplit CTAs shares an item's key tiles; the items of a sequence's last
+  // tokens come first: where the left side is not limited they have the most keys
+  const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
+  const int hgs = a.heads / g;
+  const int hg = item % hgs, b = item / hgs % a.nseq, tile2 = tiles - 1 - item / hgs / a.nseq;
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
   const int i0 = tile2 * 2 * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
   if (i0 >= ql) return;
-  const Span sp[2] = {Span(i0, tokens, ql, kl, a.left, a.right), Span(i0 + tokens, tokens, ql, kl, a.left, a.right)};
-  // key tiles of the CTA: n_sink from the front, then those of the windows
-  const int hi = sp[1].n > 0 ? sp[1].hi_max : sp[0].hi_max, lo = sp[0].lo_min;
-  const int w0 = lo / kKT;
-  const int n_sink = hi < 0 ? 0 : min(w0, (min(a.sinks, hi + 1) + kKT - 1) / kKT);
-  const int n_all = hi < 0 ? 0 : n_sink + hi / kKT - w0 + 1;
-  auto key0 = [&](int n) { return (n < n_sink ? n : w0 + n - n_sink) * kKT; };
+  Span sp0(i0, tokens, ql, kl, a.left, a.right), sp1(i0 + tokens, tokens, ql, kl, a.left, a.right);
+  const int hi_key = sp1.n > 0 ? sp1.hi_max : sp0.hi_max;
+  const Columns cols(a.sinks, sp0.lo_min);
+  sp0.shift(cols.shift());
+  sp1.shift(cols.shift());
+  const int hi = hi_key + cols.shift(), lo = sp0.lo_min;  // columns that the windows reach
+  const int n_cols = hi_key < 0 ? 0 : hi / kKT + 1;       // tiles of the item
+  const int n0 = static_cast<int>(static_cast<int64_t>(split) * n_cols / nsplit);
+  const int n_all = static_cast<int>(static_cast<int64_t>(split + 1) * n_cols / nsplit) - n0;  // and of this CTA
+  auto col0 = [&](int n) { return (n0 + n) * kKT; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -211,23 +250,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
     if (warp == 0) {
       if (lane == 0 && n_all > 0) {
-        const int nt = sp[1].n > 0 ? 2 : 1;
+        const int nt = sp1.n > 0 ? 2 : 1;
         const uint32_t q_bytes = static_cast<uint32_t>(g * tokens) * 128;  // of one 64-wide box
         mbar_arrive_expect_tx(q_full, q_bytes * (D / 64) * nt);
         for (int t = 0; t < nt; ++t)
           for (int c = 0; c < D / 64; ++c)
             tma_load_4d(sQ + t * C::kTile + c * 16384, &tmQ, q_full, c * 64, h0, i0 + t * tokens, b);
+        auto load_tile = [&](uint8_t* dst, const CUtensorMap& whole, const CUtensorMap& eight, uint64_t* bar, int v0) {
+          mbar_arrive_expect_tx(bar, C::kTile);
+          for (int c = 0; c < D / 64; ++c) {
+            if (!cols.mixed(v0)) {
+              tma_load_4d(dst + c * 16384, &whole, bar, c * 64, hk, cols.key(v0), b);
+            } else {
+              for (int j = 0; j < kKT; j += 8)
+                tma_load_4d(dst + c * 16384 + j * 128, &eight, bar, c * 64, hk, cols.key(v0 + j), b);
+            }
+          }
+        };
         for (int n = 0; n < n_all; ++n) {
           const int st = n % C::kRing;
           const uint32_t par = ((n / C::kRing) & 1) ^ 1u;
           if (!mbar_wait(&k_empty[st], par, status, kStatusTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&k_full[st], C::kTile);
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sK + st * C::kTile + c * 16384, &tmK, &k_full[st], c * 64, hk, key0(n), b);
+          load_tile(sK + st * C::kTile, tmK, tmK8, &k_full[st], col0(n));
           if (!mbar_wait(&v_empty[st], par, status, kStatusTimeoutEmpty)) break;
-          mbar_arrive_expect_tx(&v_full[st], C::kTile);
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sV + st * C::kTile + c * 16384, &tmV, &v_full[st], c * 64, hk, key0(n), b);
+          load_tile(sV + st * C::kTile, tmV, tmV8, &v_full[st], col0(n));
         }
       }
       __syncwarp();
@@ -282,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull) &&
                 mbar_wait_warp(&k_full[0], 0, status, kStatusTimeoutFull);
-      bool s0 = sp[0].sees(key0(0), a.sinks), s1 = sp[1].sees(key0(0), a.sinks);
+      bool s0 = sp0.sees(col0(0), a.sinks), s1 = sp1.sees(col0(0), a.sinks);
       if (ok && s0) ok = issue_s(0, ns0, 0);
       if (ok && s1) ok = issue_s(1, ns1, 0);
       if (ok) release(&k_empty[0]);
@@ -290,8 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = n + 1 < n_all;
         const int st = n % C::kRing, st1 = (n + 1) % C::kRing;
         const bool t0 = s0, t1 = s1;
-        s0 = more && sp[0].sees(key0(n + 1), a.sinks);
-        s1 = more && sp[1].sees(key0(n + 1), a.sinks);
+        s0 = more && sp0.sees(col0(n + 1), a.sinks);
+        s1 = more && sp1.sees(col0(n + 1), a.sinks);
         if (more) ok = mbar_wait_warp(&k_full[st1], ((n + 1) / C::kRing) & 1, status, kStatusTimeoutFull);
         if (!C::kAlias) {
           if (ok && s0) ok = issue_s(0, ns0, st1);
@@ -312,19 +358,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
     const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
-    const Span me = t == 0 ? sp[0] : sp[1];  // (an indexed array would live in local memory)
+    const Span me = t == 0 ? sp0 : sp1;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS = tmem + C::kColS + t * 128 + lanes, tP = tmem + C::kColP + t * C::kStepP + lanes;
     const uint32_t tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
     const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
-    const int row_hi = min(kl - 1, p + a.right), row_lo = p - a.left;
+    const int row_hi = min(kl - 1, p + a.right) + cols.shift(), row_lo = p - a.left + cols.shift();  // columns
     float m = -INFINITY, l = 0.f;
     int cnt = 0;
     bool ok = true;
     for (int n = 0; n < n_all && ok; ++n) {
-      const int k0 = key0(n);
-      if (!me.sees(k0, a.sinks)) continue;
+      const int v0 = col0(n);
+      if (!me.sees(v0, a.sinks)) continue;
       ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
@@ -342,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[t]);
       }
-      if (!me.whole(k0, a.sinks)) {
+      if (!me.whole(v0, a.sinks)) {
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
-        const int x1 = row_hi - k0, x0 = row_lo - k0, x2 = a.sinks - k0;
+        const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
         for (int i = 0; i < 128; ++i)
           if (i > x1 || (i < x0 && i >= x2)) s[i] = -INFINITY;
@@ -395,11 +441,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st32(tP + 32, pk[1]);
       tmem_wait_st();
       // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
-      if (k0 + kKT - 1 > hi || (k0 < lo && k0 + kKT > a.sinks)) {
+      if (v0 + kKT - 1 > hi || (v0 < lo && v0 + kKT > a.sinks)) {
         ok = mbar_wait_warp(&v_full[n % C::kRing], (n / C::kRing) & 1, status, kStatusTimeoutFull);
         if (!ok) break;
-        const int key = k0 + r;
-        if (key > hi || (key < lo && key >= a.sinks)) {
+        const int v = v0 + r;
+        if (v > hi || (v < lo && v >= a.sinks)) {
           uint4* row = reinterpret_cast<uint4*>(sV + n % C::kRing * C::kTile + r * 128);
 #pragma unroll
           for (int i = 0; i < D / 8; ++i) row[(i >> 3) * 1024 + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
@@ -415,38 +461,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
       tc_fence_after();
     }
-    // O / l, 64 columns at a time through this warp's part of its (now idle) Q tile. A row
-    // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
-    // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
-    if (__all_sync(0xffffffffu, ok) && me.n > 0) {
+    ok = __all_sync(0xffffffffu, ok);
+    if (nsplit == 1) {
+      // O / l, 64 columns at a time through this warp's part of its (now idle) Q tile. A row
+      // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
+      // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
       const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
       uint8_t* stg = sQ + t * C::kTile + q * 4096;
-      const int rows = me.n * g;
+      const int rows = ok ? me.n * g : 0;
 #pragma unroll 1
       for (int ch = 0; ch < D / 64; ++ch) {
-        uint32_t w[64];
-        if (cnt > 0) {
-          uint32_t w0_[32], w1_[32];
-          tmem_ld32(tO + 64 * ch, w0_);
-          tmem_ld32(tO + 64 * ch + 32, w1_);
-          tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            w[i] = w0_[i];
-            w[32 + i] = w1_[i];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+          take_o(tO + 64 * ch + 32 * h, cnt > 0, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 u;
+            uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              uw[j] = pack2<BF16>(__uint_as_float(w[8 * i + 2 * j]) * inv, __uint_as_float(w[8 * i + 2 * j + 1]) * inv);
+            *reinterpret_cast<uint4*>(stg + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = u;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) w[i] = 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint4 u;
-          uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            uw[j] = pack2<BF16>(__uint_as_float(w[8 * i + 2 * j]) * inv, __uint_as_float(w[8 * i + 2 * j + 1]) * inv);
-          *reinterpret_cast<uint4*>(stg + lane * 128 + ((i ^ (lane & 7)) << 4)) = u;
         }
         __syncwarp();
 #pragma unroll
@@ -459,7 +496,73 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       }
+    } else {
+      // this CTA's share of the row: O into the K / V ring (idle once both tiles' products
+      // are complete: all softmax warps come here), 16-byte chunks XOR-swizzled by row, and
+      // (m, l) into the Q tiles
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      float4* part = reinterpret_cast<float4*>(sK) + (t * 128 + r) * (D / 4);
+#pragma unroll 1
+      for (int ch = 0; ch < D / 32; ++ch) {
+        uint32_t w[32];
+        take_o(tO + 32 * ch, cnt > 0, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          part[(8 * ch + i) ^ (r & 7)] = make_float4(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]),
+                                                     __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3]));
+      }
+      reinterpret_cast<float2*>(sQ)[t * 128 + r] = make_float2(m, l);
     }
+  }
+  if (nsplit > 1) {
+    // Join the shares in rank order (the result does not depend on who finished first):
+    // with M the largest m, O = sum 2^((m_s - M) c) O_s / sum 2^((m_s - M) c) l_s. A warp
+    // takes four rows at a time, eight lanes each.
+    cluster_sync();
+    if (warp >= 4) {
+      const float c = a.scale * 1.4426950408889634f;
+      const uint32_t ml = smem_u32(sQ), part = smem_u32(sK);
+      const int sub = lane & 7;
+      for (int row = (split * 8 + warp - 4) * 4 + (lane >> 3); row < 256; row += nsplit * 32) {
+        const int t = row >> 7, r = row & 127;
+        if (r >= (t == 0 ? sp0.n : sp1.n) * g) continue;
+        float2 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < nsplit) x[i] = ld_dsmem_f2(mapa_shared(ml + row * 8, i));
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < nsplit) mx = fmaxf(mx, x[i].x);
+        float4 o[D / 32];
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (i >= nsplit) break;
+          // a share that saw no key has no weight; a NaN sum is kept
+          const float f = x[i].y != x[i].y ? 1.f : (x[i].x == -INFINITY ? 0.f : ex2((x[i].x - mx) * c));
+          sum += f * x[i].y;
+          const uint32_t src = mapa_shared(part + row * (D * 4), i);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const float4 v = ld_dsmem_f4(src + (((sub + 8 * j) ^ (r & 7)) << 4));
+            o[j].x += f * v.x;
+            o[j].y += f * v.y;
+            o[j].z += f * v.z;
+            o[j].w += f * v.w;
+          }
+        }
+        const float inv = mx == -INFINITY && sum == sum ? 0.f : 1.f / sum;
+        const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + r / g) * a.os.tok +
+                            static_cast<int64_t>(h0 + r % g) * a.os.head + 4 * sub;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + off + 32 * j) =
+              make_uint2(pack2<BF16>(o[j].x * inv, o[j].y * inv), pack2<BF16>(o[j].z * inv, o[j].w * inv));
+      }
+    }
+    cluster_sync();  // no CTA leaves while another may still read its share
   }
   tc_fence_before();
   __syncthreads();
@@ -488,8 +591,9 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   for (int d = 2; d <= 32 && d <= share; ++d)
     if (share % d == 0) g = d;
   const int tokens = 128 / g;
-  CUtensorMap tq, tk, tv;
-  if (map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
+  CUtensorMap tq, tk, tv, tk8, tv8;
+  if (map_4d(&tk8, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) ||
+      map_4d(&tv8, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) || map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
       map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT) ||
       map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT))
     return -2;
@@ -507,10 +611,38 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
   const int tiles = (a.q_len + 2 * tokens - 1) / (2 * tokens);
-  const int64_t ctas = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
-  if (ctas > 0x7fffffff) return -1;
-  k_attn_tiles<D, BF16><<<static_cast<unsigned>(ctas), kThreads, C::kSmem, s>>>(tq, tk, tv, a, g, tokens, tiles, status);
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  const int64_t items = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
+  // Split an item's key tiles over a cluster where that shortens the whole: CTAs run one an
+  // SM, so a call takes (waves of CTAs) x (tiles of a CTA + about three tiles' time of
+  // setup, and another for joining). 96 items of 51 tiles (a view of 1297 tokens, 16 heads)
+  // leave 52 SMs idle unsplit; in three, two waves of 17 tiles.
+  const int64_t span = std::min<int64_t>(a.k_len, static_cast<int64_t>(a.left) + 2 * tokens + std::min<int64_t>(a.right, a.k_len));
+  const int64_t nt = (std::min<int64_t>(a.k_len, span + a.sinks) + kKT - 1) / kKT;
+  int nsplit = 1;
+  int64_t best = 0;
+  for (int ns = 1; ns <= 8 && (ns == 1 || nt >= 4 * ns); ++ns) {
+    const int64_t cost = (items * ns + 147) / 148 * ((nt + ns - 1) / ns + 3 + (ns > 1 ? 1 : 0));
+    if (ns == 1 || cost < best) {
+      best = cost;
+      nsplit = ns;
+    }
+  }
+  if (items * nsplit > 0x7fffffff) return -1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(nsplit);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = nsplit > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_attn_tiles<D, BF16>, tq, tk, tv, tk8, tv8, a, g, tokens, tiles, nsplit, status) ==
+                 cudaSuccess
+             ? 0
+             : -4;
 }
 
 // ------------------------------------------------------------------ few queries
