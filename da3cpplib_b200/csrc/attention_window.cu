@@ -23,44 +23,51 @@ namespace da3b {
 namespace {
 
 // ------------------------------------------------------------------ many queries
-// Two tiles of 128 query rows a CTA (one CTA per SM, 12 warps), key tiles of 128 shared by
-// both. A query row is one (token, head): g query heads that share a key head lie side by
-// side, 128 / g tokens a tile, so that shared heads read their keys once and a tile spans
-// few positions (a window's ends are masked work).
-//   warp 0     TMA: both Q tiles, then the key tiles that some row sees, K and V each in a
-//              ring of its own ([128 keys][64 dims] boxes, 128B swizzle);
-//   warp 1     one thread issues S_t = Q_t K^T (M = N = 128) and O_t += P_t V (P_t from
-//              tensor memory; V is read as it lies, its dims contiguous: an MN-major operand);
-//   warps 4-7  softmax of query tile 0, warps 8-11 of tile 1: thread = row (its TMEM lane),
-//              the row's 128 scores in registers, one pass; P back to tensor memory. Two
-//              threads a row (half the keys each, maxima exchanged through shared memory)
-//              took longer: 2300 cycles a tile against 1500, as the four warps of an SM
-//              sub-partition then take their exponentials at the same time.
-// Tensor memory (512 columns): head_dim 64: S_t 128, P_t 64, O_t 64 columns each, so S_t of
-// the next key tile is issued as soon as the scores are in registers, while their
-// exponentials are taken. head_dim 128: O_t takes 128 columns and P_t lies over S_t, so
-// S_t of the next tile follows the P V product of this one.
+// Several tiles of 128 query rows a CTA (one CTA per SM) share every key tile: four with key
+// tiles of 64 at head_dim 64, two with key tiles of 128 at head_dim 128 (tensor memory: S_t
+// and O_t of every tile fill its 512 columns; P_t lies over S_t). A query row is one (token,
+// head): g query heads that share a key head lie side by side, 128 / g tokens a tile, so
+// that shared heads read their keys once and a tile spans few positions (a window's ends are
+// masked work).
+//   warp 0     TMA: the Q tiles, then the key tiles that some row sees, V of a tile together
+//              with K of the next in a ring ([keys][64 dims] boxes, 128B swizzle);
+//   warps 1-2  issue, for every other query tile each, S_t = Q_t K^T and, once P_t is there,
+//              O_t += P_t V (P_t from tensor memory; V is read as it lies, its dims
+//              contiguous: an MN-major operand) and S_t of the next key tile behind it. Few
+//              products wait in the tensor pipe's queue, so a single issuing warp's waits
+//              (about 100 cycles each, also where nothing is to be waited for) leave the pipe
+//              idle;
+//   warps 4..  softmax, four a query tile: thread = row (its TMEM lane), the row's scores in
+//              registers, one pass; P back to tensor memory.
+// A query tile is a chain (scores, exponentials, two products) that waits for itself; the
+// tiles of a CTA fill each other's waits. Two tiles at head_dim 64 ran at 716 TFLOP/s (full
+// attention, 4096 tokens): two softmax warps an SM sub-partition keep its MUFU pipe, which
+// bounds that size, half busy.
 // The maximum of a row is raised only when a tile exceeds it by more than 2^8; O_t is then
 // rescaled in tensor memory. Sums are f32 of the unrounded probabilities.
 // Masks are applied to the tiles that a window's end, the sinks' end or the last key cuts.
 // V rows of such tiles that no row of the CTA sees are zeroed in shared memory (0 * NaN).
 
-constexpr int kKT = 128;                // keys per tile
 constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the row's maximum
-constexpr int kThreads = 384;
-// Launched at 168 registers a thread (64 512 in all): the first warpgroup gives back down to
-// 72, the softmax's two warpgroups take 216.
-constexpr int kRegsLaunch = 168, kRegsCtl = 72, kRegsSoft = 216;
-static_assert(128 * kRegsCtl + 256 * kRegsSoft <= kThreads * kRegsLaunch, "register split exceeds the launch");
 
 template <int D>
 struct WinCfg {
-  static constexpr bool kAlias = D == 128;      // P over S
-  static constexpr int kTile = 128 * D * 2;     // bytes of a Q, K or V tile
-  static constexpr int kRing = D == 64 ? 4 : 2; // K tiles and V tiles in flight
-  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kRing * kTile + 256;
-  static constexpr uint32_t kColS = 0, kColP = kAlias ? 0 : 256, kStepP = kAlias ? 128 : 64;
-  static constexpr uint32_t kColO = kAlias ? 256 : 384;
+  static constexpr int kNT = D == 64 ? 4 : 2;       // query tiles
+  static constexpr int kKT = D == 64 ? 64 : 128;    // keys a tile
+  static constexpr int kThreads = 128 + 128 * kNT;
+  // registers move from the first warpgroup to the softmax's (setmaxnreg); the split may not
+  // exceed what the launch holds
+  static constexpr int kRegsLaunch = D == 64 ? 96 : 168, kRegsCtl = D == 64 ? 64 : 72, kRegsSoft = D == 64 ? 104 : 216;
+  static_assert(128 * kRegsCtl + 128 * kNT * kRegsSoft <= kThreads * kRegsLaunch, "register split");
+  static constexpr int kQTile = 128 * D * 2, kTile = kKT * D * 2;  // bytes of a Q and of a K or V tile
+  static constexpr int kRing = D == 64 ? 6 : 2;     // stages of a V tile and a K tile
+  static constexpr int kStage = 2 * kTile, kRingBytes = kRing * kStage;
+  static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 256;
+  static constexpr uint32_t kColO = kNT * kKT;
+  static_assert(kNT * (kKT + D) <= 512, "tensor memory");
+  // a CTA's share of a split item: O rows, then (m, l), over the Q tiles and the ring
+  static constexpr int kShareO = kNT * 128 * D * 4;
+  static_assert(kShareO + kNT * 128 * 8 <= kNT * kQTile + kRingBytes, "a share fits");
 };
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
@@ -99,6 +106,35 @@ __device__ __forceinline__ float2 exp2_cubic(float2 x) {
   p = __ffma2_rn(p, f, make_float2(c0, c0));
   return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// N columns of this thread's lane of tensor memory, there after tmem_wait_ld and landed.
+template <int N>
+__device__ __forceinline__ void load_cols(uint32_t taddr, float (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(s[32 * i + 0]), "=f"(s[32 * i + 1]), "=f"(s[32 * i + 2]), "=f"(s[32 * i + 3]), "=f"(s[32 * i +
+          4]), "=f"(s[32 * i + 5]), "=f"(s[32 * i + 6]), "=f"(s[32 * i + 7]), "=f"(s[32 * i + 8]), "=f"(s[32 *
+          i + 9]), "=f"(s[32 * i + 10]), "=f"(s[32 * i + 11]), "=f"(s[32 * i + 12]), "=f"(s[32 * i + 13]),
+          "=f"(s[32 * i + 14]), "=f"(s[32 * i + 15]), "=f"(s[32 * i + 16]), "=f"(s[32 * i + 17]), "=f"(s[32 *
+          i + 18]), "=f"(s[32 * i + 19]), "=f"(s[32 * i + 20]), "=f"(s[32 * i + 21]), "=f"(s[32 * i + 22]),
+          "=f"(s[32 * i + 23]), "=f"(s[32 * i + 24]), "=f"(s[32 * i + 25]), "=f"(s[32 * i + 26]), "=f"(s[32 *
+          i + 27]), "=f"(s[32 * i + 28]), "=f"(s[32 * i + 29]), "=f"(s[32 * i + 30]), "=f"(s[32 * i + 31])
+        : "r"(taddr + 32 * i));
+}
+// The lowest n bits (none for n <= 0, all for n >= 32). Masks are taken from such words:
+// compared column by column against a row's bounds, a cut tile took thousands of cycles.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Keeps every use of loaded values behind the wait before it.
+template <int N>
+__device__ __forceinline__ void landed(float (&s)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(s[i]));
 }
 
 // 32 columns of O; zeros where no product was made. Warp-collective.
@@ -153,11 +189,11 @@ struct Span {
     lo_min += by;
     lo_max += by;
   }
-  __device__ bool sees(int v0, int sinks) const {  // some key of the tile at column v0
-    return n > 0 && v0 <= hi_max && (v0 + kKT > lo_min || v0 < sinks);
+  __device__ bool sees(int v0, int keys, int sinks) const {  // some key of the tile at column v0
+    return n > 0 && v0 <= hi_max && (v0 + keys > lo_min || v0 < sinks);
   }
-  __device__ bool whole(int v0, int sinks) const {  // every row sees every key of the tile
-    return v0 + kKT - 1 <= hi_min && (v0 >= lo_max || v0 + kKT <= sinks);
+  __device__ bool whole(int v0, int keys, int sinks) const {  // every row sees every key of the tile
+    return v0 + keys - 1 <= hi_min && (v0 >= lo_max || v0 + keys <= sinks);
   }
 };
 
@@ -169,71 +205,71 @@ struct Columns {
   int front;  // columns of the sinks (0: the columns are keys from `base` on)
   int base;   // key of column `front`
   __device__ Columns(int sinks, int lo) {
-    front = sinks > lo - kKT ? 0 : (sinks + 7) & ~7;
+    front = sinks > lo - 128 ? 0 : (sinks + 7) & ~7;
     base = sinks > 0 && front == 0 ? 0 : lo;
   }
   __device__ int key(int v) const { return v < front ? v : base + v - front; }
   __device__ int shift() const { return front - base; }  // key + shift = column
-  __device__ bool mixed(int v0) const { return v0 < front && front < v0 + kKT; }
+  __device__ bool mixed(int v0, int keys) const { return v0 < front && front < v0 + keys; }
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK8,
                  const __grid_constant__ CUtensorMap tmV8, const __grid_constant__ AttnWindow a, int g, int tokens,
                  int tiles, int nsplit, int* status) {
   using C = WinCfg<D>;
+  constexpr int NT = C::kNT, KT = C::kKT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                       // [2] tiles
-  uint8_t* sK = sQ + 2 * C::kTile;          // [kRing]
-  uint8_t* sV = sK + C::kRing * C::kTile;   // [kRing]
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + C::kRing * C::kTile);
-  uint64_t* k_full = q_full + 1;            // [kRing] each
-  uint64_t* k_empty = k_full + C::kRing;
-  uint64_t* v_full = k_empty + C::kRing;
-  uint64_t* v_empty = v_full + C::kRing;
-  uint64_t* s_full = v_empty + C::kRing;    // [2] S_t complete
-  uint64_t* s_free = s_full + 2;            // [2] S_t in registers (4 warps)
-  uint64_t* p_ready = s_free + 2;           // [2] P_t written, O_t rescaled, V rows zeroed (4 warps)
-  uint64_t* pv_done = p_ready + 2;          // [2] P_t V complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  uint8_t* sQ = smem;                       // [NT]
+  // the ring: load i brings V of tile i - 1 and K of tile i (there is no tile -1 or n_all)
+  uint8_t* sKV = sQ + NT * C::kQTile;       // [kRing] V, K
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sKV + C::kRingBytes);
+  uint64_t* kv_full = q_full + 1;           // [kRing]
+  uint64_t* kv_empty = kv_full + C::kRing;  // [kRing] (both issuing warps)
+  uint64_t* s_full = kv_empty + C::kRing;   // [NT] S_t complete (and every product of t before it)
+  uint64_t* p_ready = s_full + NT;          // [NT] P_t written, O_t rescaled, V rows zeroed (4 warps)
+  uint64_t* o_full = p_ready + NT;          // [NT] the last product of O_t complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + NT);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a cluster of nsplit CTAs shares an item's key tiles; the items of a sequence's last
-  // tokens come first: where the left side is not limited they have the most keys
+  // a cluster of nsplit CTAs shares an item's key tiles; a sequence's last tokens come first:
+  // where the left side is not limited they have the most keys
   const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
   const int hgs = a.heads / g;
-  const int hg = item % hgs, b = item / hgs % a.nseq, tile2 = tiles - 1 - item / hgs / a.nseq;
+  const int tile0 = tiles - 1 - item % tiles, hg = item / tiles % hgs, b = item / tiles / hgs;
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
-  const int i0 = tile2 * 2 * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
+  const int i0 = tile0 * NT * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
   if (i0 >= ql) return;
-  Span sp0(i0, tokens, ql, kl, a.left, a.right), sp1(i0 + tokens, tokens, ql, kl, a.left, a.right);
-  const int hi_key = sp1.n > 0 ? sp1.hi_max : sp0.hi_max;
-  const Columns cols(a.sinks, sp0.lo_min);
-  sp0.shift(cols.shift());
-  sp1.shift(cols.shift());
-  const int hi = hi_key + cols.shift(), lo = sp0.lo_min;  // columns that the windows reach
-  const int n_cols = hi_key < 0 ? 0 : hi / kKT + 1;       // tiles of the item
+  const int nt = min(NT, (ql - i0 + tokens - 1) / tokens);  // query tiles with rows
+  const Span first(i0, tokens, ql, kl, a.left, a.right);
+  const Columns cols(a.sinks, first.lo_min);
+  auto span = [&](int t) {
+    Span sp(i0 + t * tokens, tokens, ql, kl, a.left, a.right);
+    sp.shift(cols.shift());
+    return sp;
+  };
+  // columns that the windows reach, tiles of the item, and of this CTA
+  const int hi_key = Span(i0 + (nt - 1) * tokens, tokens, ql, kl, a.left, a.right).hi_max;
+  const int hi = hi_key + cols.shift(), lo = first.lo_min + cols.shift();
+  const int n_cols = hi_key < 0 ? 0 : hi / KT + 1;
   const int n0 = static_cast<int>(static_cast<int64_t>(split) * n_cols / nsplit);
-  const int n_all = static_cast<int>(static_cast<int64_t>(split + 1) * n_cols / nsplit) - n0;  // and of this CTA
-  auto col0 = [&](int n) { return (n0 + n) * kKT; };
+  const int n_all = static_cast<int>(static_cast<int64_t>(split + 1) * n_cols / nsplit) - n0;
+  auto col0 = [&](int n) { return (n0 + n) * KT; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < C::kRing; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NT; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_free[t], 4);
       mbar_init(&p_ready[t], 4);
-      mbar_init(&pv_done[t], 1);
+      mbar_init(&o_full[t], 1);
     }
     fence_mbar_init();
     prefetch_tmap(&tmQ);
@@ -247,184 +283,174 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsCtl));
     if (warp == 0) {
       if (lane == 0 && n_all > 0) {
-        const int nt = sp1.n > 0 ? 2 : 1;
         const uint32_t q_bytes = static_cast<uint32_t>(g * tokens) * 128;  // of one 64-wide box
         mbar_arrive_expect_tx(q_full, q_bytes * (D / 64) * nt);
         for (int t = 0; t < nt; ++t)
           for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sQ + t * C::kTile + c * 16384, &tmQ, q_full, c * 64, h0, i0 + t * tokens, b);
+            tma_load_4d(sQ + t * C::kQTile + c * 16384, &tmQ, q_full, c * 64, h0, i0 + t * tokens, b);
         auto load_tile = [&](uint8_t* dst, const CUtensorMap& whole, const CUtensorMap& eight, uint64_t* bar, int v0) {
-          mbar_arrive_expect_tx(bar, C::kTile);
           for (int c = 0; c < D / 64; ++c) {
-            if (!cols.mixed(v0)) {
-              tma_load_4d(dst + c * 16384, &whole, bar, c * 64, hk, cols.key(v0), b);
+            if (!cols.mixed(v0, KT)) {
+              tma_load_4d(dst + c * KT * 128, &whole, bar, c * 64, hk, cols.key(v0), b);
             } else {
-              for (int j = 0; j < kKT; j += 8)
-                tma_load_4d(dst + c * 16384 + j * 128, &eight, bar, c * 64, hk, cols.key(v0 + j), b);
+              for (int j = 0; j < KT; j += 8)
+                tma_load_4d(dst + (c * KT + j) * 128, &eight, bar, c * 64, hk, cols.key(v0 + j), b);
             }
           }
         };
-        for (int n = 0; n < n_all; ++n) {
-          const int st = n % C::kRing;
-          const uint32_t par = ((n / C::kRing) & 1) ^ 1u;
-          if (!mbar_wait(&k_empty[st], par, status, kStatusTimeoutEmpty)) break;
-          load_tile(sK + st * C::kTile, tmK, tmK8, &k_full[st], col0(n));
-          if (!mbar_wait(&v_empty[st], par, status, kStatusTimeoutEmpty)) break;
-          load_tile(sV + st * C::kTile, tmV, tmV8, &v_full[st], col0(n));
+        int st = 0;
+        uint32_t par = 1;
+        for (int i = 0; i <= n_all; ++i) {
+          if (!mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty)) break;
+          uint8_t* dst = sKV + st * C::kStage;
+          mbar_arrive_expect_tx(&kv_full[st], i == 0 || i == n_all ? C::kTile : C::kStage);
+          if (i < n_all) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], col0(i));
+          if (i > 0) load_tile(dst, tmV, tmV8, &kv_full[st], col0(i - 1));
+          if (++st == C::kRing) { st = 0; par ^= 1u; }
         }
       }
       __syncwarp();
-    } else if (warp == 1 && n_all > 0) {
+    } else if (warp < 3 && n_all > 0) {
       // The whole warp runs this loop and one elected lane issues: addresses and descriptors
-      // then stay in uniform registers, where the instructions want them. With one lane in
-      // the loop every product's operands were moved there one by one, and the issuing
-      // thread, not the softmax or the tensor pipe, set the pace (3900 cycles a key tile).
+      // then stay in uniform registers, where the instructions want them. (With one lane in
+      // the loop every product's operands were moved there one by one, and that set the
+      // pace.)
       constexpr uint32_t fmt = BF16 ? (1u << 7) | (1u << 10) : 0u;
-      constexpr uint32_t id_s = umma_idesc_f16(128, kKT) | fmt;
+      constexpr uint32_t id_s = umma_idesc_f16(128, KT) | fmt;
       constexpr uint32_t id_o = umma_idesc_f16(128, D) | fmt | (1u << 16);  // B is MN-major
+      constexpr int kMine = NT / 2;  // query tiles of this warp: t = warp - 1 + 2 j
       const bool one = elect_one();
-      const uint64_t qd0 = umma_desc_sw128(smem_u32(sQ)), kd0 = umma_desc_sw128(smem_u32(sK));
-      const uint64_t vd0 = desc_mn_sw128(smem_u32(sV), 16384);
-      int ns0 = 0, ns1 = 0, np0 = 0, np1 = 0;  // S and P V products issued
-      auto issue_s = [&](int t, int& ns, int st) -> bool {
-        if (!C::kAlias && ns > 0 && !mbar_wait_warp(&s_free[t], (ns - 1) & 1, status, kStatusTimeoutAccumFree))
-          return false;
-        tc_fence_after();
-        const uint64_t qd = qd0 + t * (C::kTile >> 4), kd = kd0 + st * (C::kTile >> 4);
+      const int tw = warp - 1;
+      const uint64_t qd0 = umma_desc_sw128(smem_u32(sQ) + tw * C::kQTile);
+      const uint64_t vd0 = desc_mn_sw128(smem_u32(sKV), KT * 128), kd0 = umma_desc_sw128(smem_u32(sKV) + C::kTile);
+      const uint32_t ts0 = tmem + tw * KT, to0 = tmem + C::kColO + tw * D;
+      auto issue_s = [&](int j, int st) {
+        const uint64_t qd = qd0 + j * (2 * C::kQTile >> 4), kd = kd0 + st * (C::kStage >> 4);
         if (one) {
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tmem + C::kColS + t * 128, qd + c * 1024 + 2 * kk, kd + c * 1024 + 2 * kk, id_s,
+              umma_f16(ts0 + 2 * j * KT, qd + c * 1024 + 2 * kk, kd + c * (KT * 8) + 2 * kk, id_s,
                        (c > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&s_full[t]);
+          umma_commit(&s_full[tw + 2 * j]);
         }
         __syncwarp();
-        ++ns;
-        return true;
       };
-      auto issue_pv = [&](int t, int& np, int st) -> bool {
-        if (!mbar_wait_warp(&p_ready[t], np & 1, status, kStatusTimeoutFull)) return false;
-        tc_fence_after();
-        const uint64_t vd = vd0 + st * (C::kTile >> 4);
-        if (one) {
-#pragma unroll
-          for (int kk = 0; kk < kKT / 16; ++kk)
-            umma_f16_tmem_a(tmem + C::kColO + t * D, tmem + C::kColP + t * C::kStepP + 8 * kk, vd + 128 * kk, id_o,
-                            (np > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&pv_done[t]);
-        }
-        __syncwarp();
-        ++np;
-        return true;
+      const Span sp0 = span(tw), sp1 = span(tw + 2 * (kMine - 1));
+      auto seen = [&](int n) {  // bit j: some row of tile j sees key tile n
+        uint32_t bits = sp0.sees(col0(n), KT, a.sinks) ? 1u : 0u;
+        if (kMine > 1 && sp1.sees(col0(n), KT, a.sinks)) bits |= 2u;
+        return bits;
       };
-      auto release = [&](uint64_t* bar) {
-        if (one) umma_commit(bar);
-        __syncwarp();
-      };
+      uint32_t now = seen(0), next = 0, made = 0, parity = 0;  // made: a product into O was issued
       bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull) &&
-                mbar_wait_warp(&k_full[0], 0, status, kStatusTimeoutFull);
-      bool s0 = sp0.sees(col0(0), a.sinks), s1 = sp1.sees(col0(0), a.sinks);
-      if (ok && s0) ok = issue_s(0, ns0, 0);
-      if (ok && s1) ok = issue_s(1, ns1, 0);
-      if (ok) release(&k_empty[0]);
-      for (int n = 0; n < n_all && ok; ++n) {
-        const bool more = n + 1 < n_all;
-        const int st = n % C::kRing, st1 = (n + 1) % C::kRing;
-        const bool t0 = s0, t1 = s1;
-        s0 = more && sp0.sees(col0(n + 1), a.sinks);
-        s1 = more && sp1.sees(col0(n + 1), a.sinks);
-        if (more) ok = mbar_wait_warp(&k_full[st1], ((n + 1) / C::kRing) & 1, status, kStatusTimeoutFull);
-        if (!C::kAlias) {
-          if (ok && s0) ok = issue_s(0, ns0, st1);
-          if (ok && s1) ok = issue_s(1, ns1, st1);
-          if (ok && more) release(&k_empty[st1]);
-        }
-        if (ok) ok = mbar_wait_warp(&v_full[st], (n / C::kRing) & 1, status, kStatusTimeoutFull);
-        if (ok && t0) ok = issue_pv(0, np0, st);
-        if (C::kAlias && ok && s0) ok = issue_s(0, ns0, st1);
-        if (ok && t1) ok = issue_pv(1, np1, st);
-        if (C::kAlias && ok && s1) ok = issue_s(1, ns1, st1);
-        if (ok) {
-          release(&v_empty[st]);
-          if (C::kAlias && more) release(&k_empty[st1]);
-        }
+                mbar_wait_warp(&kv_full[0], 0, status, kStatusTimeoutFull);
+      if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < kMine; ++j)
+          if (now >> j & 1) issue_s(j, 0);
+        if (one) umma_commit(&kv_empty[0]);
+        __syncwarp();
       }
+      int st = 1 % C::kRing;
+      uint32_t par = C::kRing == 1;
+      for (int n = 0; n < n_all && ok; ++n) {
+        next = n + 1 < n_all ? seen(n + 1) : 0;
+        ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
+        const uint64_t vd = vd0 + st * (C::kStage >> 4);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+          if (ok && (now >> j & 1)) {
+            ok = mbar_wait_warp(&p_ready[tw + 2 * j], parity >> j & 1, status, kStatusTimeoutFull);
+            if (ok) {
+              tc_fence_after();
+              const uint32_t add = made >> j & 1;
+              if (one) {
+#pragma unroll
+                for (int kk = 0; kk < KT / 16; ++kk)
+                  umma_f16_tmem_a(to0 + 2 * j * D, ts0 + 2 * j * KT + 8 * kk, vd + 128 * kk, id_o, kk > 0 ? 1u : add);
+              }
+              __syncwarp();
+              made |= 1u << j;
+              parity ^= 1u << j;
+            }
+          }
+          if (ok && (next >> j & 1)) issue_s(j, st);
+        }
+        if (ok && one) umma_commit(&kv_empty[st]);
+        __syncwarp();
+        now = next;
+        if (++st == C::kRing) { st = 0; par ^= 1u; }
+      }
+      if (ok && one) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) umma_commit(&o_full[tw + 2 * j]);
+      }
+      __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
-    const Span me = t == 0 ? sp0 : sp1;
+    const Span me = span(t);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tS = tmem + C::kColS + t * 128 + lanes, tP = tmem + C::kColP + t * C::kStepP + lanes;
-    const uint32_t tO = tmem + C::kColO + t * D + lanes;
+    const uint32_t tS = tmem + t * KT + lanes, tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
     const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
     const int row_hi = min(kl - 1, p + a.right) + cols.shift(), row_lo = p - a.left + cols.shift();  // columns
     float m = -INFINITY, l = 0.f;
-    int cnt = 0;
+    int cnt = 0, st = 0;
+    uint32_t par = 0;
     bool ok = true;
     for (int n = 0; n < n_all && ok; ++n) {
       const int v0 = col0(n);
-      if (!me.sees(v0, a.sinks)) continue;
+      if (++st == C::kRing) { st = 0; par ^= 1u; }  // the stage of this tile's V
+      if (!me.sees(v0, KT, a.sinks)) continue;
+      // S_t of this tile was issued behind the last P V product: O_t and P_t are free too
       ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
-      float s[128];
+      float s[KT];
+      load_cols<KT>(tS, s);
+      // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
+      if (v0 + KT - 1 > hi || (v0 < lo && v0 + KT > a.sinks)) {
+        ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
+        if (!ok) break;
+        const int v = v0 + r;
+        if (r < KT && (v > hi || (v < lo && v >= a.sinks))) {
+          uint4* row = reinterpret_cast<uint4*>(sKV + st * C::kStage + r * 128);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[32];
-        tmem_ld32(tS + 32 * i, w);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[32 * i + j] = __uint_as_float(w[j]);
+          for (int i = 0; i < D / 8; ++i) row[(i >> 3) * (KT * 8) + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
       }
       tmem_wait_ld();
-      if (!C::kAlias) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
-      }
-      if (!me.whole(v0, a.sinks)) {
+      landed<KT>(s);
+      if (!me.whole(v0, KT, a.sinks)) {
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
         const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i > x1 || (i < x0 && i >= x2)) s[i] = -INFINITY;
+        for (int w = 0; w < KT / 32; ++w) {
+          const uint32_t bits = below(x1 + 1 - 32 * w) & (~below(x0 - 32 * w) | below(x2 - 32 * w));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[32 * w + i] = bits >> i & 1u ? s[32 * w + i] : -INFINITY;
+        }
       }
       float m8[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[120 + i]);
+      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[KT - 8 + i]);
 #pragma unroll
-      for (int i = 8; i < 120; i += 16)
+      for (int i = 8; i < KT - 8; i += 16)
 #pragma unroll
         for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
       const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
       const bool raise = cnt == 0 || (mt - m) * c > kRaise;
-      const float alpha = raise ? ex2((m - mt) * c) : 1.f;
-      if (raise) m = mt;
-      const float mc = m == -INFINITY ? 0.f : m * c;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      uint32_t pk[2][32];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) {
-        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(-mc, -mc));
-        const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
-        sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-        pk[i >> 5][i & 31] = pack2<BF16>(e.x, e.y);
-      }
-      const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-      // P of the last tile has been read and O_t is complete (with P over S, S_t of this
-      // tile was issued after that product); only now, behind the exponentials
-      if (!C::kAlias && cnt > 0) {
-        ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
-        if (!ok) break;
-        tc_fence_after();
-      }
       if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
+        const float alpha = raise ? ex2((m - mt) * c) : 1.f;
 #pragma unroll 1
         for (int i = 0; i < D; i += 16) {
           uint32_t w[16];
@@ -436,29 +462,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l *= alpha;
       }
-      l += s2.x + s2.y;
-      tmem_st32(tP, pk[0]);
-      tmem_st32(tP + 32, pk[1]);
-      tmem_wait_st();
-      // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
-      if (v0 + kKT - 1 > hi || (v0 < lo && v0 + kKT > a.sinks)) {
-        ok = mbar_wait_warp(&v_full[n % C::kRing], (n / C::kRing) & 1, status, kStatusTimeoutFull);
-        if (!ok) break;
-        const int v = v0 + r;
-        if (v > hi || (v < lo && v >= a.sinks)) {
-          uint4* row = reinterpret_cast<uint4*>(sV + n % C::kRing * C::kTile + r * 128);
+      if (raise) m = mt;
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) row[(i >> 3) * 1024 + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
+      for (int h = 0; h < KT / 64; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), make_float2(c, c),
+                                      make_float2(-mc, -mc));
+          const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
+          sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+          pk[i] = pack2<BF16>(e.x, e.y);
         }
-        fence_proxy_async_smem();
+        tmem_st32(tS + 32 * h, pk);
       }
+      const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+      l += s2.x + s2.y;
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t]);
       ++cnt;
     }
     if (ok && cnt > 0) {
-      ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+      ok = mbar_wait_warp(&o_full[t], 0, status, kStatusTimeoutAccum);
       tc_fence_after();
     }
     ok = __all_sync(0xffffffffu, ok);
@@ -467,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
       // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
       const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
-      uint8_t* stg = sQ + t * C::kTile + q * 4096;
+      uint8_t* stg = sQ + t * C::kQTile + q * 4096;
       const int rows = ok ? me.n * g : 0;
 #pragma unroll 1
       for (int ch = 0; ch < D / 64; ++ch) {
@@ -497,11 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     } else {
-      // this CTA's share of the row: O into the K / V ring (idle once both tiles' products
-      // are complete: all softmax warps come here), 16-byte chunks XOR-swizzled by row, and
-      // (m, l) into the Q tiles
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      float4* part = reinterpret_cast<float4*>(sK) + (t * 128 + r) * (D / 4);
+      // this CTA's share of the row, over the Q tiles and the ring (idle once every tile's
+      // products are complete: all softmax warps come here): O, 16-byte chunks XOR-swizzled
+      // by row, then (m, l)
+      asm volatile("bar.sync 1, %0;" ::"n"(128 * NT) : "memory");
+      float4* part = reinterpret_cast<float4*>(smem) + (t * 128 + r) * (D / 4);
 #pragma unroll 1
       for (int ch = 0; ch < D / 32; ++ch) {
         uint32_t w[32];
@@ -511,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           part[(8 * ch + i) ^ (r & 7)] = make_float4(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]),
                                                      __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3]));
       }
-      reinterpret_cast<float2*>(sQ)[t * 128 + r] = make_float2(m, l);
+      reinterpret_cast<float2*>(smem + C::kShareO)[t * 128 + r] = make_float2(m, l);
     }
   }
   if (nsplit > 1) {
@@ -521,11 +550,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();
     if (warp >= 4) {
       const float c = a.scale * 1.4426950408889634f;
-      const uint32_t ml = smem_u32(sQ), part = smem_u32(sK);
+      const uint32_t part = smem_u32(smem), ml = part + C::kShareO;
       const int sub = lane & 7;
-      for (int row = (split * 8 + warp - 4) * 4 + (lane >> 3); row < 256; row += nsplit * 32) {
+      const int last = ((nt - 1) * 128) + min(tokens, ql - i0 - (nt - 1) * tokens) * g;
+      for (int row = (split * 4 * NT + warp - 4) * 4 + (lane >> 3); row < last; row += nsplit * 16 * NT) {
         const int t = row >> 7, r = row & 127;
-        if (r >= (t == 0 ? sp0.n : sp1.n) * g) continue;
+        if (r >= tokens * g) continue;
         float2 x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -582,6 +612,32 @@ int map_4d(CUtensorMap* m, const void* p, const Strides& st, int bf16, int D, in
   return make_tmap_4d(m, p, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, strides, box);
 }
 
+// Clusters of ns CTAs of the tiled kernel that the device holds at once (asked once each).
+template <int D, bool BF16>
+int clusters_at_once(int ns, int dev) {
+  using C = WinCfg<D>;
+  static std::atomic<int> known[64][9];
+  int n = known[dev & 63][ns].load(std::memory_order_relaxed);
+  if (n == 0 && ns == 1) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    known[dev & 63][ns].store(n, std::memory_order_relaxed);
+  } else if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ns));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ns);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, k_attn_tiles<D, BF16>, &cfg) != cudaSuccess || n <= 0) n = -1;
+    known[dev & 63][ns].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 template <int D, bool BF16>
 int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   using C = WinCfg<D>;
@@ -594,8 +650,8 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   CUtensorMap tq, tk, tv, tk8, tv8;
   if (map_4d(&tk8, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) ||
       map_4d(&tv8, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) || map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
-      map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT) ||
-      map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, kKT))
+      map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, C::kKT) ||
+      map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, C::kKT))
     return -2;
   static std::atomic<uint64_t> attr_set{0};  // one bit per device; first calls may race
   int dev = 0;
@@ -606,23 +662,25 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
     // the register split waits for registers that the launch must have
     cudaFuncAttributes fa;
     if (cudaFuncGetAttributes(&fa, k_attn_tiles<D, BF16>) != cudaSuccess ||
-        fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsSoft)
+        fa.numRegs * C::kThreads < 128 * C::kRegsCtl + 128 * C::kNT * C::kRegsSoft)
       return -5;
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
-  const int tiles = (a.q_len + 2 * tokens - 1) / (2 * tokens);
+  const int tiles = (a.q_len + C::kNT * tokens - 1) / (C::kNT * tokens);
   const int64_t items = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
   // Split an item's key tiles over a cluster where that shortens the whole: CTAs run one an
-  // SM, so a call takes (waves of CTAs) x (tiles of a CTA + about three tiles' time of
-  // setup, and another for joining). 96 items of 51 tiles (a view of 1297 tokens, 16 heads)
-  // leave 52 SMs idle unsplit; in three, two waves of 17 tiles.
-  const int64_t span = std::min<int64_t>(a.k_len, static_cast<int64_t>(a.left) + 2 * tokens + std::min<int64_t>(a.right, a.k_len));
-  const int64_t nt = (std::min<int64_t>(a.k_len, span + a.sinks) + kKT - 1) / kKT;
+  // SM, so a call takes its waves of CTAs times a CTA's time, with the times measured (ns):
+  // 48 items of 102 key tiles (a view of 1297 tokens, 16 heads) leave 100 SMs idle unsplit.
+  constexpr int64_t kTileNs = D == 64 ? 550 : 1900, kSetupNs = 4000, kJoinNs = 5000;
+  const int64_t reach = std::min<int64_t>(a.k_len, static_cast<int64_t>(a.left) + C::kNT * tokens + std::min(a.right, a.q_len));
+  const int64_t nt = (std::min<int64_t>(a.k_len, reach + a.sinks) + C::kKT - 1) / C::kKT;
   int nsplit = 1;
   int64_t best = 0;
   for (int ns = 1; ns <= 8 && (ns == 1 || nt >= 4 * ns); ++ns) {
-    const int64_t cost = (items * ns + 147) / 148 * ((nt + ns - 1) / ns + 3 + (ns > 1 ? 1 : 0));
-    if (ns == 1 || cost < best) {
+    const int64_t at_once = clusters_at_once<D, BF16>(ns, dev);
+    if (at_once <= 0) continue;
+    const int64_t cost = (items + at_once - 1) / at_once * ((nt + ns - 1) / ns * kTileNs + kSetupNs + (ns > 1 ? kJoinNs : 0));
+    if (best == 0 || cost < best) {
       best = cost;
       nsplit = ns;
     }
@@ -630,7 +688,7 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   if (items * nsplit > 0x7fffffff) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
