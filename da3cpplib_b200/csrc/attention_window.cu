@@ -23,26 +23,23 @@ namespace da3b {
 namespace {
 
 // ------------------------------------------------------------------ many queries
-// Several tiles of 128 query rows a CTA (one CTA per SM) share every key tile: four with key
-// tiles of 64 at head_dim 64, two with key tiles of 128 at head_dim 128 (tensor memory: S_t
-// and O_t of every tile fill its 512 columns; P_t lies over S_t). A query row is one (token,
-// head): g query heads that share a key head lie side by side, 128 / g tokens a tile, so
-// that shared heads read their keys once and a tile spans few positions (a window's ends are
-// masked work).
+// Several tiles of 128 query rows a CTA (one CTA per SM) share every key tile: three at
+// head_dim 64, two at 128. A query row is one (token, head): g query heads that share a key
+// head lie side by side, 128 / g tokens a tile, so that shared heads read their keys once
+// and a tile spans few positions (a window's ends are masked work).
 //   warp 0     TMA: the Q tiles, then the key tiles that some row sees, V of a tile together
 //              with K of the next in a ring ([keys][64 dims] boxes, 128B swizzle);
-//   warps 1-2  issue, for every other query tile each, S_t = Q_t K^T and, once P_t is there,
-//              O_t += P_t V (P_t from tensor memory; V is read as it lies, its dims
-//              contiguous: an MN-major operand) and S_t of the next key tile behind it. Few
-//              products wait in the tensor pipe's queue, so a single issuing warp's waits
-//              (about 100 cycles each, also where nothing is to be waited for) leave the pipe
-//              idle;
+//   warps 1..  one a query tile: S_t = Q_t K^T of the next key tile as soon as the last
+//              scores are in registers, and O_t += P_t V once P_t is there (P_t from tensor
+//              memory; V is read as it lies, its dims contiguous: an MN-major operand);
 //   warps 4..  softmax, four a query tile: thread = row (its TMEM lane), the row's scores in
 //              registers, one pass; P back to tensor memory.
-// A query tile is a chain (scores, exponentials, two products) that waits for itself; the
-// tiles of a CTA fill each other's waits. Two tiles at head_dim 64 ran at 716 TFLOP/s (full
-// attention, 4096 tokens): two softmax warps an SM sub-partition keep its MUFU pipe, which
-// bounds that size, half busy.
+// What a query tile waits for is hidden twice: its next scores are made while it takes its
+// exponentials (S_t and P_t have columns of their own: with P_t over S_t the two products
+// followed the softmax, a turn of 1880 cycles for 64 keys), and the other tiles fill the
+// rest. Each tile has an issuing warp of its own because few products wait in the tensor
+// pipe's queue: one warp's waits (about 100 cycles each, also where nothing is to be waited
+// for) leave the pipe idle.
 // The maximum of a row is raised only when a tile exceeds it by more than 2^8; O_t is then
 // rescaled in tensor memory. Sums are f32 of the unrounded probabilities.
 // Masks are applied to the tiles that a window's end, the sinks' end or the last key cuts.
@@ -52,19 +49,19 @@ constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the r
 
 template <int D>
 struct WinCfg {
-  static constexpr int kNT = D == 64 ? 4 : 2;       // query tiles
-  static constexpr int kKT = D == 64 ? 64 : 128;    // keys a tile
+  static constexpr int kNT = D == 64 ? 3 : 2;  // query tiles
+  static constexpr int kKT = 64;               // keys a tile
   static constexpr int kThreads = 128 + 128 * kNT;
   // registers move from the first warpgroup to the softmax's (setmaxnreg); the split may not
   // exceed what the launch holds
-  static constexpr int kRegsLaunch = D == 64 ? 96 : 168, kRegsCtl = D == 64 ? 64 : 72, kRegsSoft = D == 64 ? 104 : 216;
+  static constexpr int kRegsLaunch = D == 64 ? 128 : 168, kRegsCtl = D == 64 ? 80 : 72, kRegsSoft = D == 64 ? 144 : 216;
   static_assert(128 * kRegsCtl + 128 * kNT * kRegsSoft <= kThreads * kRegsLaunch, "register split");
   static constexpr int kQTile = 128 * D * 2, kTile = kKT * D * 2;  // bytes of a Q and of a K or V tile
-  static constexpr int kRing = D == 64 ? 6 : 2;     // stages of a V tile and a K tile
+  static constexpr int kRing = D == 64 ? 8 : 4;     // stages of a V tile and a K tile
   static constexpr int kStage = 2 * kTile, kRingBytes = kRing * kStage;
   static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 256;
-  static constexpr uint32_t kColO = kNT * kKT;
-  static_assert(kNT * (kKT + D) <= 512, "tensor memory");
+  static constexpr uint32_t kColP = kNT * kKT, kColO = kColP + kNT * kKT / 2;  // behind S_t
+  static_assert(kColO + kNT * D <= 512, "tensor memory");
   // a CTA's share of a split item: O rows, then (m, l), over the Q tiles and the ring
   static constexpr int kShareO = kNT * 128 * D * 4;
   static_assert(kShareO + kNT * 128 * 8 <= kNT * kQTile + kRingBytes, "a share fits");
@@ -189,12 +186,23 @@ struct Span {
     lo_min += by;
     lo_max += by;
   }
-  __device__ bool sees(int v0, int keys, int sinks) const {  // some key of the tile at column v0
-    return n > 0 && v0 <= hi_max && (v0 + keys > lo_min || v0 < sinks);
+};
+
+// The same in key tiles of KT columns: which a query tile sees, and sees whole.
+template <int KT>
+struct Seen {
+  int first, last, front;           // some row sees tiles [first, last] and [0, front), up to last
+  int whole0, whole1, whole_front;  // every row sees all of [whole0, whole1] and [0, whole_front), up to whole1
+  __device__ Seen(const Span& sp, int sinks) {
+    first = sp.lo_min / KT;
+    last = sp.n > 0 && sp.hi_max >= 0 ? sp.hi_max / KT : -1;
+    front = sinks / KT + (sinks % KT != 0);
+    whole0 = sp.lo_max / KT + (sp.lo_max % KT != 0);
+    whole1 = sp.hi_min >= 0 ? (sp.hi_min + 1) / KT - 1 : -1;
+    whole_front = sinks / KT;
   }
-  __device__ bool whole(int v0, int keys, int sinks) const {  // every row sees every key of the tile
-    return v0 + keys - 1 <= hi_min && (v0 >= lo_max || v0 + keys <= sinks);
-  }
+  __device__ bool some(int tile) const { return tile <= last && (tile >= first || tile < front); }
+  __device__ bool whole(int tile) const { return tile <= whole1 && (tile >= whole0 || tile < whole_front); }
 };
 
 // The keys of a CTA as one run of columns: the sinks, up to a multiple of eight, then the
@@ -218,7 +226,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK8,
                  const __grid_constant__ CUtensorMap tmV8, const __grid_constant__ AttnWindow a, int g, int tokens,
-                 int tiles, int nsplit, int* status) {
+                 int qt, int tiles, int nsplit, int* status) {
   using C = WinCfg<D>;
   constexpr int NT = C::kNT, KT = C::kKT;
   extern __shared__ uint8_t smem_raw[];
@@ -228,11 +236,12 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   uint8_t* sKV = sQ + NT * C::kQTile;       // [kRing] V, K
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sKV + C::kRingBytes);
   uint64_t* kv_full = q_full + 1;           // [kRing]
-  uint64_t* kv_empty = kv_full + C::kRing;  // [kRing] (both issuing warps)
-  uint64_t* s_full = kv_empty + C::kRing;   // [NT] S_t complete (and every product of t before it)
-  uint64_t* p_ready = s_full + NT;          // [NT] P_t written, O_t rescaled, V rows zeroed (4 warps)
-  uint64_t* o_full = p_ready + NT;          // [NT] the last product of O_t complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + NT);
+  uint64_t* kv_empty = kv_full + C::kRing;  // [kRing] (every issuing warp)
+  uint64_t* s_full = kv_empty + C::kRing;   // [NT] S_t complete
+  uint64_t* s_free = s_full + NT;           // [NT] S_t in registers (4 warps)
+  uint64_t* p_ready = s_free + NT;          // [NT] P_t written, O_t rescaled, V rows zeroed (4 warps)
+  uint64_t* pv_done = p_ready + NT;         // [NT] P_t V complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NT);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a cluster of nsplit CTAs shares an item's key tiles; a sequence's last tokens come first:
@@ -242,13 +251,13 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   const int tile0 = tiles - 1 - item % tiles, hg = item / tiles % hgs, b = item / tiles / hgs;
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
-  const int i0 = tile0 * NT * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
+  const int i0 = tile0 * qt * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
   if (i0 >= ql) return;
-  const int nt = min(NT, (ql - i0 + tokens - 1) / tokens);  // query tiles with rows
+  const int nt = min(qt, (ql - i0 + tokens - 1) / tokens);  // query tiles with rows
   const Span first(i0, tokens, ql, kl, a.left, a.right);
   const Columns cols(a.sinks, first.lo_min);
   auto span = [&](int t) {
-    Span sp(i0 + t * tokens, tokens, ql, kl, a.left, a.right);
+    Span sp(i0 + t * tokens, t < nt ? tokens : 0, ql, kl, a.left, a.right);
     sp.shift(cols.shift());
     return sp;
   };
@@ -264,12 +273,13 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     mbar_init(q_full, 1);
     for (int s = 0; s < C::kRing; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 2);
+      mbar_init(&kv_empty[s], NT);
     }
     for (int t = 0; t < NT; ++t) {
       mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], 4);
       mbar_init(&p_ready[t], 4);
-      mbar_init(&o_full[t], 1);
+      mbar_init(&pv_done[t], 1);
     }
     fence_mbar_init();
     prefetch_tmap(&tmQ);
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         }
       }
       __syncwarp();
-    } else if (warp < 3 && n_all > 0) {
+    } else if (warp <= NT && n_all > 0) {
       // The whole warp runs this loop and one elected lane issues: addresses and descriptors
       // then stay in uniform registers, where the instructions want them. (With one lane in
       // the loop every product's operands were moved there one by one, and that set the
@@ -321,84 +331,79 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       constexpr uint32_t fmt = BF16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t id_s = umma_idesc_f16(128, KT) | fmt;
       constexpr uint32_t id_o = umma_idesc_f16(128, D) | fmt | (1u << 16);  // B is MN-major
-      constexpr int kMine = NT / 2;  // query tiles of this warp: t = warp - 1 + 2 j
       const bool one = elect_one();
-      const int tw = warp - 1;
-      const uint64_t qd0 = umma_desc_sw128(smem_u32(sQ) + tw * C::kQTile);
+      const int t = warp - 1;
+      const uint64_t qd = umma_desc_sw128(smem_u32(sQ) + t * C::kQTile);
       const uint64_t vd0 = desc_mn_sw128(smem_u32(sKV), KT * 128), kd0 = umma_desc_sw128(smem_u32(sKV) + C::kTile);
-      const uint32_t ts0 = tmem + tw * KT, to0 = tmem + C::kColO + tw * D;
-      auto issue_s = [&](int j, int st) {
-        const uint64_t qd = qd0 + j * (2 * C::kQTile >> 4), kd = kd0 + st * (C::kStage >> 4);
+      const uint32_t tS = tmem + t * KT, tP = tmem + C::kColP + t * (KT / 2), tO = tmem + C::kColO + t * D;
+      const Seen<KT> see(span(t), a.sinks);
+      auto issue_s = [&](int st) {
+        const uint64_t kd = kd0 + st * (C::kStage >> 4);
         if (one) {
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(ts0 + 2 * j * KT, qd + c * 1024 + 2 * kk, kd + c * (KT * 8) + 2 * kk, id_s,
-                       (c > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&s_full[tw + 2 * j]);
+              umma_f16(tS, qd + c * 1024 + 2 * kk, kd + c * (KT * 8) + 2 * kk, id_s, (c > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&s_full[t]);
         }
         __syncwarp();
       };
-      const Span sp0 = span(tw), sp1 = span(tw + 2 * (kMine - 1));
-      auto seen = [&](int n) {  // bit j: some row of tile j sees key tile n
-        uint32_t bits = sp0.sees(col0(n), KT, a.sinks) ? 1u : 0u;
-        if (kMine > 1 && sp1.sees(col0(n), KT, a.sinks)) bits |= 2u;
-        return bits;
-      };
-      uint32_t now = seen(0), next = 0, made = 0, parity = 0;  // made: a product into O was issued
       bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull) &&
                 mbar_wait_warp(&kv_full[0], 0, status, kStatusTimeoutFull);
+      bool now = see.some(n0);
+      int ns = 0, np = 0;  // S and P V products issued
       if (ok) {
         tc_fence_after();
-#pragma unroll
-        for (int j = 0; j < kMine; ++j)
-          if (now >> j & 1) issue_s(j, 0);
+        if (now) {
+          issue_s(0);
+          ++ns;
+        }
         if (one) umma_commit(&kv_empty[0]);
         __syncwarp();
       }
       int st = 1 % C::kRing;
       uint32_t par = C::kRing == 1;
       for (int n = 0; n < n_all && ok; ++n) {
-        next = n + 1 < n_all ? seen(n + 1) : 0;
+        const bool next = n + 1 < n_all && see.some(n0 + n + 1);
         ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
-        const uint64_t vd = vd0 + st * (C::kStage >> 4);
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) {
-          if (ok && (now >> j & 1)) {
-            ok = mbar_wait_warp(&p_ready[tw + 2 * j], parity >> j & 1, status, kStatusTimeoutFull);
-            if (ok) {
-              tc_fence_after();
-              const uint32_t add = made >> j & 1;
-              if (one) {
-#pragma unroll
-                for (int kk = 0; kk < KT / 16; ++kk)
-                  umma_f16_tmem_a(to0 + 2 * j * D, ts0 + 2 * j * KT + 8 * kk, vd + 128 * kk, id_o, kk > 0 ? 1u : add);
-              }
-              __syncwarp();
-              made |= 1u << j;
-              parity ^= 1u << j;
-            }
+        if (ok && next) {
+          if (ns > 0) ok = mbar_wait_warp(&s_free[t], (ns - 1) & 1, status, kStatusTimeoutAccumFree);
+          if (ok) {
+            tc_fence_after();
+            issue_s(st);
+            ++ns;
           }
-          if (ok && (next >> j & 1)) issue_s(j, st);
+        }
+        if (ok && now) {
+          ok = mbar_wait_warp(&p_ready[t], np & 1, status, kStatusTimeoutFull);
+          if (ok) {
+            tc_fence_after();
+            const uint64_t vd = vd0 + st * (C::kStage >> 4);
+            if (one) {
+#pragma unroll
+              for (int kk = 0; kk < KT / 16; ++kk)
+                umma_f16_tmem_a(tO, tP + 8 * kk, vd + 128 * kk, id_o, (np > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&pv_done[t]);
+            }
+            __syncwarp();
+            ++np;
+          }
         }
         if (ok && one) umma_commit(&kv_empty[st]);
         __syncwarp();
         now = next;
         if (++st == C::kRing) { st = 0; par ^= 1u; }
       }
-      if (ok && one) {
-#pragma unroll
-        for (int j = 0; j < kMine; ++j) umma_commit(&o_full[tw + 2 * j]);
-      }
-      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
-    const Span me = span(t);
+    const Seen<KT> see(span(t), a.sinks);
+    const int fix0 = lo > a.sinks ? a.sinks / KT : 1, fix1 = lo > a.sinks ? (lo - 1) / KT : 0;  // tiles with unseen keys,
+    const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;                                         // and the last
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tS = tmem + t * KT + lanes, tO = tmem + C::kColO + t * D + lanes;
+    const uint32_t tS = tmem + t * KT + lanes, tP = tmem + C::kColP + t * (KT / 2) + lanes, tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
     const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
     const int row_hi = min(kl - 1, p + a.right) + cols.shift(), row_lo = p - a.left + cols.shift();  // columns
@@ -409,15 +414,14 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     for (int n = 0; n < n_all && ok; ++n) {
       const int v0 = col0(n);
       if (++st == C::kRing) { st = 0; par ^= 1u; }  // the stage of this tile's V
-      if (!me.sees(v0, KT, a.sinks)) continue;
-      // S_t of this tile was issued behind the last P V product: O_t and P_t are free too
+      if (!see.some(n0 + n)) continue;
       ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
       float s[KT];
       load_cols<KT>(tS, s);
       // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
-      if (v0 + KT - 1 > hi || (v0 < lo && v0 + KT > a.sinks)) {
+      if (n0 + n == fix2 || (n0 + n >= fix0 && n0 + n <= fix1)) {
         ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
         if (!ok) break;
         const int v = v0 + r;
@@ -430,7 +434,10 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       }
       tmem_wait_ld();
       landed<KT>(s);
-      if (!me.whole(v0, KT, a.sinks)) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_free[t]);
+      if (!see.whole(n0 + n)) {
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
         const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
@@ -449,37 +456,39 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
       const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
       const bool raise = cnt == 0 || (mt - m) * c > kRaise;
-      if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
-        const float alpha = raise ? ex2((m - mt) * c) : 1.f;
-#pragma unroll 1
-        for (int i = 0; i < D; i += 16) {
-          uint32_t w[16];
-          tmem_ld16(tO + i, w);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
-          tmem_st16(tO + i, w);
-        }
-        l *= alpha;
-      }
+      const float alpha = raise ? ex2((m - mt) * c) : 1.f;
       if (raise) m = mt;
       const float mc = m == -INFINITY ? 0.f : m * c;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      uint32_t pk[KT / 2];
 #pragma unroll
-      for (int h = 0; h < KT / 64; ++h) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 x = __ffma2_rn(make_float2(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), make_float2(c, c),
-                                      make_float2(-mc, -mc));
-          const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
-          sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-          pk[i] = pack2<BF16>(e.x, e.y);
-        }
-        tmem_st32(tS + 32 * h, pk);
+      for (int i = 0; i < KT / 2; ++i) {
+        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(-mc, -mc));
+        const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
+        sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+        pk[i] = pack2<BF16>(e.x, e.y);
       }
       const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+      // behind the exponentials: P of the last tile has been read, and O_t is complete
+      if (cnt > 0) {
+        ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+        if (!ok) break;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+          for (int i = 0; i < D; i += 16) {
+            uint32_t w[16];
+            tmem_ld16(tO + i, w);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+            tmem_st16(tO + i, w);
+          }
+          l *= alpha;
+        }
+      }
       l += s2.x + s2.y;
+      tmem_st32(tP, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       ++cnt;
     }
     if (ok && cnt > 0) {
-      ok = mbar_wait_warp(&o_full[t], 0, status, kStatusTimeoutAccum);
+      ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
       tc_fence_after();
     }
     ok = __all_sync(0xffffffffu, ok);
@@ -497,7 +506,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
       const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
       uint8_t* stg = sQ + t * C::kQTile + q * 4096;
-      const int rows = ok ? me.n * g : 0;
+      const int rows = ok ? span(t).n * g : 0;
 #pragma unroll 1
       for (int ch = 0; ch < D / 64; ++ch) {
 #pragma unroll
@@ -666,25 +675,33 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
       return -5;
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
-  const int tiles = (a.q_len + C::kNT * tokens - 1) / (C::kNT * tokens);
-  const int64_t items = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
-  // Split an item's key tiles over a cluster where that shortens the whole: CTAs run one an
-  // SM, so a call takes its waves of CTAs times a CTA's time, with the times measured (ns):
-  // 48 items of 102 key tiles (a view of 1297 tokens, 16 heads) leave 100 SMs idle unsplit.
-  constexpr int64_t kTileNs = D == 64 ? 550 : 1900, kSetupNs = 4000, kJoinNs = 5000;
-  const int64_t reach = std::min<int64_t>(a.k_len, static_cast<int64_t>(a.left) + C::kNT * tokens + std::min(a.right, a.q_len));
-  const int64_t nt = (std::min<int64_t>(a.k_len, reach + a.sinks) + C::kKT - 1) / C::kKT;
-  int nsplit = 1;
+  // Query tiles a CTA, and a split of its key tiles over a cluster: whatever makes the call
+  // shortest. CTAs run one an SM, so a call takes its waves of CTAs times a CTA's time, with
+  // the times measured (ns a key tile for 1, 2, .. query tiles). A view of 1297 tokens and 16
+  // heads over 7800 keys: 48 items of four tiles leave 100 SMs idle unsplit, and two thirds
+  // of them in two; 64 items of three tiles in two fill 128.
+  constexpr int64_t kTileNs[2][3] = {{700, 800, 950}, {800, 950, 0}};
+  constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
+  int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
-  for (int ns = 1; ns <= 8 && (ns == 1 || nt >= 4 * ns); ++ns) {
-    const int64_t at_once = clusters_at_once<D, BF16>(ns, dev);
-    if (at_once <= 0) continue;
-    const int64_t cost = (items + at_once - 1) / at_once * ((nt + ns - 1) / ns * kTileNs + kSetupNs + (ns > 1 ? kJoinNs : 0));
-    if (best == 0 || cost < best) {
-      best = cost;
-      nsplit = ns;
+  for (int n = C::kNT; n >= 1; --n) {
+    const int64_t items = static_cast<int64_t>((a.q_len + n * tokens - 1) / (n * tokens)) * (a.heads / g) * a.nseq;
+    const int64_t reach = std::min<int64_t>(a.k_len, static_cast<int64_t>(a.left) + n * tokens + std::min(a.right, a.q_len));
+    const int64_t keys = (std::min<int64_t>(a.k_len, reach + a.sinks) + C::kKT - 1) / C::kKT;  // key tiles
+    for (int ns = 1; ns <= 8 && (ns == 1 || keys >= 4 * ns); ++ns) {
+      const int64_t at_once = clusters_at_once<D, BF16>(ns, dev);
+      if (at_once <= 0) continue;
+      const int64_t cost = (items + at_once - 1) / at_once *
+                           ((keys + ns - 1) / ns * kTileNs[D == 128][n - 1] + kSetupNs + (ns > 1 ? kJoinNs : 0));
+      if (best == 0 || cost < best) {
+        best = cost;
+        nsplit = ns;
+        qt = n;
+      }
     }
   }
+  const int tiles = (a.q_len + qt * tokens - 1) / (qt * tokens);
+  const int64_t items = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
   if (items * nsplit > 0x7fffffff) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
@@ -697,7 +714,8 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = nsplit > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_attn_tiles<D, BF16>, tq, tk, tv, tk8, tv8, a, g, tokens, tiles, nsplit, status) ==
+  return cudaLaunchKernelEx(&cfg, k_attn_tiles<D, BF16>, tq, tk, tv, tk8, tv8, a, g, tokens, qt, tiles, nsplit,
+                            status) ==
                  cudaSuccess
              ? 0
              : -4;
