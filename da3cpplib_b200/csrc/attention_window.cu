@@ -400,8 +400,11 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
     const Seen<KT> see(span(t), a.sinks);
-    const int fix0 = lo > a.sinks ? a.sinks / KT : 1, fix1 = lo > a.sinks ? (lo - 1) / KT : 0;  // tiles with unseen keys,
-    const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;                                         // and the last
+    // tiles with keys that no row of the CTA sees, and the tiles that need no look: seen whole
+    // by this query tile, and by its windows alone
+    const int fix0 = lo > a.sinks ? a.sinks / KT : 1, fix1 = lo > a.sinks ? (lo - 1) / KT : 0;
+    const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;
+    const int plain0 = max(see.whole0, fix1 + 1), plain1 = min(min(see.whole1, see.last), fix2 < 0 ? see.whole1 : fix2 - 1);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS = tmem + t * KT + lanes, tP = tmem + C::kColP + t * (KT / 2) + lanes, tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
@@ -412,16 +415,17 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     uint32_t par = 0;
     bool ok = true;
     for (int n = 0; n < n_all && ok; ++n) {
-      const int v0 = col0(n);
       if (++st == C::kRing) { st = 0; par ^= 1u; }  // the stage of this tile's V
-      if (!see.some(n0 + n)) continue;
+      const bool plain = n0 + n >= plain0 && n0 + n <= plain1;
+      if (!plain && !see.some(n0 + n)) continue;
+      const int v0 = col0(n);
       ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
       float s[KT];
       load_cols<KT>(tS, s);
       // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
-      if (n0 + n == fix2 || (n0 + n >= fix0 && n0 + n <= fix1)) {
+      if (!plain && (n0 + n == fix2 || (n0 + n >= fix0 && n0 + n <= fix1))) {
         ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
         if (!ok) break;
         const int v = v0 + r;
@@ -437,7 +441,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_free[t]);
-      if (!see.whole(n0 + n)) {
+      if (!plain && !see.whole(n0 + n)) {
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
         const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
@@ -680,7 +684,7 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   // the times measured (ns a key tile for 1, 2, .. query tiles). A view of 1297 tokens and 16
   // heads over 7800 keys: 48 items of four tiles leave 100 SMs idle unsplit, and two thirds
   // of them in two; 64 items of three tiles in two fill 128.
-  constexpr int64_t kTileNs[2][3] = {{700, 800, 950}, {800, 950, 0}};
+  constexpr int64_t kTileNs[2][3] = {{750, 1050, 1250}, {780, 1070, 0}};
   constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
   int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
