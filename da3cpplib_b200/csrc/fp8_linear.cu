@@ -16,8 +16,10 @@
 //              x 4 columns, one word = a row's four blocks) and issues four MMAs (K = 32)
 //              a k-block, selecting the block's byte by the descriptor's scale ids;
 //   warps 4-19 epilogue: tensor memory -> registers (64 columns a thread, row = lane) ->
-//              bias, activation, quantisation -> 64-byte row pieces through a swizzled
-//              staging buffer, so that four lanes store consecutive bytes of a row. Four
+//              bias, activation, quantisation -> 64-byte row pieces in a swizzled staging
+//              buffer, stored (or, onto the residual, added) by TMA: the load-store unit,
+//              73 % busy with the pieces' reads and stores when the warps made them, only
+//              writes the buffer. Four
 //              warps an SM sub-partition hide each other's latencies: with eight warps of
 //              128 columns, M = 87680, K = 1024, N = 4096 with GELU took 528-580 us.
 // Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
@@ -46,8 +48,8 @@ constexpr int kThreads = 640;
 constexpr int kRegsLaunch = 96, kRegsCtl = 40, kRegsEpi = 104;
 static_assert(128 * kRegsCtl + 512 * kRegsEpi <= kThreads * kRegsLaunch, "register split exceeds the launch");
 constexpr int kEpiWarps = 16;
-constexpr int kStageOut = 2048;                  // a warp's staging buffer, [32 rows][64 B]
-constexpr int kEpiWarpBytes = kStageOut + 3 * 256;  // + bias and scale of 64 columns, 32 maxima (x 2)
+constexpr int kStageOut = 2048;     // a warp's staging buffer, [32 rows][64 B], 64B swizzle
+constexpr int kEpiTab = 3 * 256;    // a warp's bias and scale of 64 columns, 32 maxima (x 2)
 constexpr int kSfBuffers = 8;  // scale buffers in tensor memory
 
 // CG = 1: a CTA computes 128 x 128, two accumulators, the two halves of the epilogue warps
@@ -66,7 +68,7 @@ struct Cfg {
   static constexpr int kAcc = CG == 2 ? 1 : 2;
   static constexpr int kSfCols = 4 * (kSfATiles + kSfBTiles);
   static constexpr uint32_t kColSf = kAcc * kBN;
-  static constexpr int kEpiBytes = kEpiWarps * kEpiWarpBytes;
+  static constexpr int kEpiBytes = kEpiWarps * (kStageOut + kEpiTab);
   static constexpr int kSmem = 1024 + kStages * (kStageBytes + kSfBytes) + kEpiBytes + 256;
   static_assert(kColSf + kSfBuffers * kSfCols <= 512, "tensor memory");
   // A scale buffer is reused kSfBuffers groups later, and a k-block's MMAs start only when
@@ -163,65 +165,54 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 // A warp's [32 rows][64 B] piece of the output: lane = row holds 16 words; rows [m0, m0 +
-// 32), columns from n0 on. Through the warp's staging buffer (16-byte chunks XOR-swizzled
-// by row), so that four lanes write 64 consecutive bytes of a row. Where the output is not
-// 16-byte aligned, or at its last columns, element by element.
+// 32), columns from n0 on. Into the warp's staging buffer (16-byte chunks XOR-swizzled by
+// row, the 64B swizzle), then out by TMA, which clips it at the last row, and at the last
+// column where that ends a 16-byte chunk (it writes whole chunks). Another last piece, and an
+// output whose rows are not 16-byte aligned, is written from the buffer element by element.
 // ESZ: bytes an element; RESID: out += value (f32).
 template <int ESZ, bool RESID>
-__device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, const uint32_t (&words)[16], int m0, int n0,
-                                            bool vec, int lane) {
+__device__ __forceinline__ void store_piece(const Fp8Linear& a, const CUtensorMap* map, uint8_t* stg,
+                                            const uint32_t (&words)[16], int m0, int n0, bool tma, int lane) {
+  if (n0 >= a.N) return;
+  if (tma) {
+    if (lane == 0) bulk_wait_read<0>();  // the last piece has left the buffer
+    __syncwarp();
+    tma = n0 + 64 / ESZ <= a.N || a.N * ESZ % 16 == 0;
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *reinterpret_cast<uint4*>(stg + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
         make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
-  __syncwarp();
-  const int c = lane & 3, n = n0 + c * (16 / ESZ);
-  const size_t pitch = static_cast<size_t>(a.ldo) * ESZ;
-  if (vec && n + 16 / ESZ <= a.N) {
-    uint8_t* col = static_cast<uint8_t*>(a.out) + static_cast<size_t>(n) * ESZ;
-    uint4 old[4];
-    if (RESID) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int m = m0 + 8 * k + (lane >> 2);
-        if (m < a.M) old[k] = *reinterpret_cast<const uint4*>(col + m * pitch);
-      }
+  if (tma) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (RESID) tma_reduce_add_2d(map, stg, n0, m0);
+      else tma_store_2d(map, stg, n0, m0);
+      bulk_commit();
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int row = 8 * k + (lane >> 2), m = m0 + row;
-      uint4 u = *reinterpret_cast<const uint4*>(stg + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-      if (RESID) {
-        u.x = __float_as_uint(__uint_as_float(u.x) + __uint_as_float(old[k].x));
-        u.y = __float_as_uint(__uint_as_float(u.y) + __uint_as_float(old[k].y));
-        u.z = __float_as_uint(__uint_as_float(u.z) + __uint_as_float(old[k].z));
-        u.w = __float_as_uint(__uint_as_float(u.w) + __uint_as_float(old[k].w));
-      }
-      if (m < a.M) *reinterpret_cast<uint4*>(col + m * pitch) = u;
-    }
+    return;
   }
-  // every 16-byte chunk was stored above, or is stored here element by element, 32
-  // consecutive elements a store
-  const int n_vec = vec ? a.N / (16 / ESZ) * (16 / ESZ) : 0;
-  if (n0 + 64 / ESZ > n_vec) {
-    const int rows = min(32, a.M - m0);
-    uint8_t* out = static_cast<uint8_t*>(a.out) + m0 * pitch;
+  __syncwarp();
+  // 32 consecutive elements a store
+  const size_t pitch = static_cast<size_t>(a.ldo) * ESZ;
+  const int rows = min(32, a.M - m0);
+  uint8_t* out = static_cast<uint8_t*>(a.out) + m0 * pitch;
 #pragma unroll 4
-    for (int row = 0; row < rows; ++row) {
+  for (int row = 0; row < rows; ++row) {
 #pragma unroll
-      for (int e = lane; e < 64 / ESZ; e += 32) {
-        const int ne = n0 + e, b = e * ESZ;
-        if (ne < n_vec || ne >= a.N) continue;
-        const uint8_t* src = stg + row * 64 + (((b >> 4) ^ ((row >> 1) & 3)) << 4) + (b & 15);
-        uint8_t* o = out + row * pitch + static_cast<size_t>(ne) * ESZ;
-        if (ESZ == 4) {
-          const float v = *reinterpret_cast<const float*>(src);
-          *reinterpret_cast<float*>(o) = RESID ? *reinterpret_cast<const float*>(o) + v : v;
-        } else if (ESZ == 2) {
-          *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(src);
-        } else {
-          *o = *src;
-        }
+    for (int e = lane; e < 64 / ESZ; e += 32) {
+      const int ne = n0 + e, b = e * ESZ;
+      if (ne >= a.N) continue;
+      const uint8_t* src = stg + row * 64 + (((b >> 4) ^ ((row >> 1) & 3)) << 4) + (b & 15);
+      uint8_t* o = out + row * pitch + static_cast<size_t>(ne) * ESZ;
+      if (ESZ == 4) {
+        const float v = *reinterpret_cast<const float*>(src);
+        *reinterpret_cast<float*>(o) = RESID ? *reinterpret_cast<const float*>(o) + v : v;
+      } else if (ESZ == 2) {
+        *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(src);
+      } else {
+        *o = *src;
       }
     }
   }
@@ -233,9 +224,9 @@ __device__ __forceinline__ void store_piece(const Fp8Linear& a, uint8_t* stg, co
 // it shares with the warp that has the other 64 columns of the block, [2][32]: `other` is
 // that warp's table, `pair` the barrier of the two, `flip` alternates with the tiles. False if
 // a wait ran out.
-__device__ __forceinline__ bool epilogue64(const Fp8Linear& a, float (&v)[64], int m0, int n0, uint8_t* stg, float* ctab,
-                                           const float* other, uint64_t* pair, uint32_t flip, bool vec, int lane,
-                                           int* status) {
+__device__ __forceinline__ bool epilogue64(const Fp8Linear& a, const CUtensorMap* map, float (&v)[64], int m0, int n0,
+                                           uint8_t* stg, float* ctab, const float* other, uint64_t* pair, uint32_t flip,
+                                           bool tma, int lane, int* status) {
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
     const float4 b = *reinterpret_cast<const float4*>(ctab + i);
@@ -262,7 +253,7 @@ __device__ __forceinline__ bool epilogue64(const Fp8Linear& a, float (&v)[64], i
 #pragma unroll
         for (int i = 0; i < 16; ++i) words[i] = pack_bf16(v[32 * p + 2 * i], v[32 * p + 2 * i + 1]);
       }
-      store_piece<2, false>(a, stg, words, m0, n0 + 32 * p, vec, lane);
+      store_piece<2, false>(a, map, stg, words, m0, n0 + 32 * p, tma, lane);
     }
   } else if (a.kind == kFp8OutQ) {
     // this warp's 64 columns and its partner's are one block of the output's scales;
@@ -283,18 +274,18 @@ __device__ __forceinline__ bool epilogue64(const Fp8Linear& a, float (&v)[64], i
                            fp8_nan_if_inf(v[4 * i + 2]) * inv, fp8_nan_if_inf(v[4 * i + 3]) * inv);
     if (m0 + lane < a.M && (n0 & 127) == 0)
       a.out_scales[fp8_scale_offset(m0 + lane, n0 >> 7, (a.M + 127) / 128)] = static_cast<uint8_t>(byte);
-    store_piece<1, false>(a, stg, words, m0, n0, vec, lane);
+    store_piece<1, false>(a, map, stg, words, m0, n0, tma, lane);
   } else {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       if (a.kind == kFp8OutResid) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) words[i] = __float_as_uint(v[16 * p + i] * ctab[64 + 16 * p + i]);
-        store_piece<4, true>(a, stg, words, m0, n0 + 16 * p, vec, lane);
+        store_piece<4, true>(a, map, stg, words, m0, n0 + 16 * p, tma, lane);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) words[i] = __float_as_uint(v[16 * p + i]);
-        store_piece<4, false>(a, stg, words, m0, n0 + 16 * p, vec, lane);
+        store_piece<4, false>(a, map, stg, words, m0, n0 + 16 * p, tma, lane);
       }
     }
   }
@@ -305,7 +296,7 @@ template <int CG>
 __global__ void __launch_bounds__(kThreads, 1)
     k_fp8_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-               const __grid_constant__ Fp8Linear a, int vec, int* status) {
+               const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Fp8Linear a, int tma, int* status) {
   using C = Cfg<CG>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -434,10 +425,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter, 64-column part of the tile
     const int cols = (CG == 2 ? part : part & 1) * 64;
-    uint8_t* stg = sEpi + (warp - 4) * kEpiWarpBytes;
-    float* ctab = reinterpret_cast<float*>(stg + kStageOut);
+    uint8_t* stg = sEpi + (warp - 4) * kStageOut;
+    uint8_t* tabs = sEpi + kEpiWarps * kStageOut;
+    float* ctab = reinterpret_cast<float*>(tabs + (warp - 4) * kEpiTab);
     // the warp with the other half of a 128-column block: the next or last part
-    const float* other = reinterpret_cast<const float*>(sEpi + ((warp - 4) ^ 4) * kEpiWarpBytes + kStageOut);
+    const float* other = reinterpret_cast<const float*>(tabs + ((warp - 4) ^ 4) * kEpiTab);
     uint64_t* pair = &pairs[q + 4 * (part >> 1)];
     uint32_t uses = 0;
     int it = 0;
@@ -474,9 +466,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // whole 128-column blocks are in or out together, so both warps of a pair come here
       if (m0 < a.M && (n0 & ~127) < a.N &&
-          !epilogue64(a, v, m0, n0, stg, ctab, other, pair, uses++ & 1, vec != 0, lane, status))
+          !epilogue64(a, &tmC, v, m0, n0, stg, ctab, other, pair, uses++ & 1, tma != 0, lane, status))
         break;
     }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -538,7 +532,15 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
   const long m_units = ((a.M + 127) / 128 + CG - 1) / CG;
   const long tiles = m_units * ((a.N + C::kBN - 1) / C::kBN);
   if (tiles > 0x7fffffffL) return -1;
-  const int vec = aligned(a.out, 16) && (static_cast<size_t>(a.ldo) * out_size(a.kind)) % 16 == 0;
+  const int esz = out_size(a.kind);
+  const int tma = aligned(a.out, 16) && (static_cast<size_t>(a.ldo) * esz) % 16 == 0;
+  CUtensorMap tc = tsa;
+  if (tma && make_tmap_2d_typed(&tc, a.out,
+                                esz == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                : esz == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                                esz, a.M, a.N, a.ldo, 64 / esz, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+    return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<long>(tiles, sm_count(dev) / CG) * CG));
   cfg.blockDim = dim3(kThreads);
@@ -550,7 +552,7 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_fp8_gemm<CG>, ta, tb, tsa, tsb, a, vec, status) == cudaSuccess ? 0 : -4;
+  return cudaLaunchKernelEx(&cfg, k_fp8_gemm<CG>, ta, tb, tsa, tsb, tc, a, tma, status) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace
