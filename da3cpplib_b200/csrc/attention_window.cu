@@ -15,6 +15,7 @@
 
 #include "attention_window.h"
 #include "da3b.h"
+#include "launch.h"
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   // where the left side is not limited they have the most keys
   const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
   const int hgs = a.heads / g;
+  pdl_wait();
   const int tile0 = tiles - 1 - item % tiles, hg = item / tiles % hgs, b = item / tiles / hgs;
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
@@ -707,19 +709,8 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   const int tiles = (a.q_len + qt * tokens - 1) / (qt * tokens);
   const int64_t items = static_cast<int64_t>(tiles) * (a.heads / g) * a.nseq;
   if (items * nsplit > 0x7fffffff) return -1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
-  cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(nsplit);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = nsplit > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_attn_tiles<D, BF16>, tq, tk, tv, tk8, tv8, a, g, tokens, qt, tiles, nsplit,
-                            status) ==
+  return launch_pdl(k_attn_tiles<D, BF16>, dim3(static_cast<unsigned>(items * nsplit)), C::kThreads, C::kSmem, s,
+                    static_cast<unsigned>(nsplit), tq, tk, tv, tk8, tv8, a, g, tokens, qt, tiles, nsplit, status) ==
                  cudaSuccess
              ? 0
              : -4;
@@ -782,6 +773,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
   const int hk = item % a.kv_heads, b = item / a.kv_heads;
   const int share = a.heads / a.kv_heads;
+  pdl_wait();
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
   const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
   const int rows = ql * share;
@@ -1044,18 +1036,10 @@ int launch_few(const AttnWindow& a, int* status, cudaStream_t s) {
   const int64_t tiles = (std::min<int64_t>(a.k_len, window) + kFewKeys - 1) / kFewKeys;
   const int nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 296 / items, tiles / 4})));
   if (items * nsplit > 0x7fffffff) return -1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * nsplit));
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(nsplit);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = nsplit > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_attn_few<D, BF16>, tk, tv, a, nsplit, status) == cudaSuccess ? 0 : -4;
+  return launch_pdl(k_attn_few<D, BF16>, dim3(static_cast<unsigned>(items * nsplit)), kFewThreads, C::kSmem, s,
+                    static_cast<unsigned>(nsplit), tk, tv, a, nsplit, status) == cudaSuccess
+             ? 0
+             : -4;
 }
 
 // No keys at all (k_len 0; a tensor map cannot be empty): zeros in the rows that count.

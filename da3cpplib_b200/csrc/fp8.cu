@@ -5,13 +5,14 @@
 // byte are written. Eight threads share a block of 128 columns (16 consecutive values
 // each), so the block's maximum takes three shuffles, the codes leave as one 16-byte
 // store a thread, and 32 threads together hold the four blocks of one scale word.
-#include <algorithm>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "da3b.h"
 #include "fp8.cuh"
 #include "fp8.h"
+#include "launch.h"
+#include "ptx.cuh"
 
 namespace da3b {
 
@@ -100,7 +101,9 @@ __global__ void __launch_bounds__(256)
     k_quantize_fp8(const T* __restrict__ x, int rows, int K, int ldx, uint8_t* __restrict__ q, int ldq,
                    uint8_t* __restrict__ scales) {
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_trigger();
   if (r >= rows) return;
+  pdl_wait();
   const int row_tiles = (rows + 127) / 128, c0 = blockIdx.y * 1024, lane = threadIdx.x & 31;
   const T* row = x + static_cast<size_t>(r) * ldx;
   float v[16], w[16];
@@ -123,7 +126,9 @@ __global__ void __launch_bounds__(256)
   __shared__ float part[2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = WARPS == 1 ? blockIdx.x * 8 + warp : blockIdx.x;
+  pdl_trigger();
   if (WARPS == 1 && r >= rows) return;
+  pdl_wait();
   const int sub = WARPS == 1 ? 0 : warp;
   const float* row = x + static_cast<size_t>(r) * ldx;
   float v[NV][16];
@@ -189,11 +194,12 @@ int launch_quantize(const void* xv, int rows, int K, int ldx, uint8_t* q, int ld
   if (reinterpret_cast<uintptr_t>(x) % sizeof(T)) return -1;
   const dim3 grid((static_cast<unsigned>(rows) + 7) / 8, (static_cast<unsigned>(K) + 1023) / 1024);
   if (grid.y > 65535) return -1;
+  cudaError_t e;
   if (K % 16 == 0 && (static_cast<size_t>(ldx) * sizeof(T)) % 32 == 0 && aligned32(x))
-    k_quantize_fp8<T, true><<<grid, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
+    e = launch_pdl(k_quantize_fp8<T, true>, grid, 256, 0, s, 1, x, rows, K, ldx, q, ldq, scales);
   else
-    k_quantize_fp8<T, false><<<grid, 256, 0, s>>>(x, rows, K, ldx, q, ldq, scales);
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+    e = launch_pdl(k_quantize_fp8<T, false>, grid, 256, 0, s, 1, x, rows, K, ldx, q, ldq, scales);
+  return e == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace
@@ -218,10 +224,13 @@ int layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g, cons
   if (rows == 0) return 0;
   const bool vec = K % 16 == 0 && ldx % 8 == 0 && aligned32(x) && aligned32(g) && aligned32(b);
   const unsigned per_warp = static_cast<unsigned>((rows + 7) / 8), per_block = static_cast<unsigned>(rows);
-#define DA3B_LNF8(W, NV, GRID)                                                                          \
-  do {                                                                                                  \
-    if (vec) k_layernorm_fp8<W, NV, true><<<GRID, 256, 0, s>>>(x, rows, K, ldx, g, b, eps, q, ldq, scales); \
-    else k_layernorm_fp8<W, NV, false><<<GRID, 256, 0, s>>>(x, rows, K, ldx, g, b, eps, q, ldq, scales);    \
+  cudaError_t e;
+#define DA3B_LNF8(W, NV, GRID)                                                                                        \
+  do {                                                                                                                \
+    if (vec) e = launch_pdl(k_layernorm_fp8<W, NV, true>, dim3(GRID), 256, 0, s, 1, x, rows, K, ldx, g, b, eps, q,    \
+                            ldq, scales);                                                                             \
+    else e = launch_pdl(k_layernorm_fp8<W, NV, false>, dim3(GRID), 256, 0, s, 1, x, rows, K, ldx, g, b, eps, q, ldq,  \
+                        scales);                                                                                      \
   } while (0)
   if (K <= 512) DA3B_LNF8(1, 1, per_warp);
   else if (K <= 1024) DA3B_LNF8(1, 2, per_warp);
@@ -229,7 +238,7 @@ int layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g, cons
   else if (K <= 8192) DA3B_LNF8(8, 2, per_block);
   else DA3B_LNF8(8, 4, per_block);
 #undef DA3B_LNF8
-  return cudaGetLastError() == cudaSuccess ? 0 : -4;
+  return e == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace da3b

@@ -35,6 +35,7 @@
 #include "fp8.cuh"
 #include "fp8.h"
 #include "gemm.h"
+#include "launch.h"
 #include "ops.h"
 #include "ptx.cuh"
 
@@ -54,13 +55,14 @@ constexpr int kSfBuffers = 8;  // scale buffers in tensor memory
 
 // CG = 1: a CTA computes 128 x 128, two accumulators, the two halves of the epilogue warps
 // take alternate tiles. CG = 2: a CTA pair computes 256 x 256 (128 x 256 in each CTA's
-// tensor memory), one accumulator that all epilogue warps read at once: the scales need
-// tensor memory too, so a second 256-column accumulator does not fit.
+// tensor memory, half of the w tile in each CTA's ring), one accumulator that all epilogue
+// warps read at once: the scales need tensor memory too, so a second 256-column accumulator
+// does not fit.
 template <int CG>
 struct Cfg {
-  static constexpr int kBN = CG == 2 ? 256 : 128;
+  static constexpr int kBN = 128 * CG;
   static constexpr int kABytes = 128 * 128;
-  static constexpr int kBBytes = 128 * 128;  // each CTA of a pair holds half of the w tile
+  static constexpr int kBBytes = 128 * 128;
   static constexpr int kSfATiles = 1, kSfBTiles = kBN / 128;
   static constexpr int kSfBytes = 512 * (kSfATiles + kSfBTiles);
   static constexpr int kStageBytes = kABytes + kBBytes;
@@ -222,10 +224,10 @@ __device__ __forceinline__ void store_piece(const Fp8Linear& a, const CUtensorMa
 // Epilogue of a warp's 32 rows x 64 columns held as v (lane = row m0 + lane, column n0 + i).
 // ctab: the warp's copies of bias and scale for these columns, [2][64], and the row maxima
 // it shares with the warp that has the other 64 columns of the block, [2][32]: `other` is
-// that warp's table, `pair` the barrier of the two, `flip` alternates with the tiles. False if
-// a wait ran out.
+// that warp's table, `pair` the barrier of the two, `uses` its phases so far. False if a wait
+// ran out.
 __device__ __forceinline__ bool epilogue64(const Fp8Linear& a, const CUtensorMap* map, float (&v)[64], int m0, int n0,
-                                           uint8_t* stg, float* ctab, const float* other, uint64_t* pair, uint32_t flip,
+                                           uint8_t* stg, float* ctab, const float* other, uint64_t* pair, uint32_t& uses,
                                            bool tma, int lane, int* status) {
 #pragma unroll
   for (int i = 0; i < 64; i += 4) {
@@ -237,7 +239,7 @@ __device__ __forceinline__ bool epilogue64(const Fp8Linear& a, const CUtensorMap
   }
   if (a.act == kActRelu) {
 #pragma unroll
-    for (int i = 0; i < 64; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // NaN stays NaN
+    for (int i = 0; i < 64; ++i) asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(v[i]));  // NaN stays NaN
   } else if (a.act != kActNone) {
 #pragma unroll
     for (int i = 0; i < 64; i += 8) gelu8(v + i);
@@ -257,21 +259,35 @@ __device__ __forceinline__ bool epilogue64(const Fp8Linear& a, const CUtensorMap
     }
   } else if (a.kind == kFp8OutQ) {
     // this warp's 64 columns and its partner's are one block of the output's scales;
-    // columns past N are zero (w has no rows there, and their bias is zero)
+    // columns past N are zero (w has no rows there, and their bias is zero). Infinities are
+    // looked for once the maximum is known: both warps of a pair then see one, and do it again.
     float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) amax = fmaxf(amax, finite_abs(v[i]));
-    ctab[128 + 32 * flip + lane] = amax;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(pair);
-    if (!mbar_wait_warp(pair, flip, status, kStatusTimeoutAccum)) return false;
-    amax = fmaxf(amax, other[128 + 32 * flip + lane]);
+    for (int i = 0; i < 64; ++i) amax = fmaxf(amax, fabsf(v[i]));
+    auto swap = [&]() -> bool {
+      const uint32_t flip = uses++ & 1;
+      ctab[128 + 32 * flip + lane] = amax;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pair);
+      if (!mbar_wait_warp(pair, flip, status, kStatusTimeoutAccum)) return false;
+      amax = fmaxf(amax, other[128 + 32 * flip + lane]);
+      return true;
+    };
+    if (!swap()) return false;
+    if (__any_sync(0xffffffffu, amax > kFltMax)) {
+      amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        amax = fmaxf(amax, finite_abs(v[i]));
+        v[i] = fp8_nan_if_inf(v[i]);
+      }
+      if (!swap()) return false;
+    }
     const uint32_t byte = fp8_scale_byte(amax);
     const float inv = fp8_inv_scale(byte);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      words[i] = fp8_pack4(fp8_nan_if_inf(v[4 * i]) * inv, fp8_nan_if_inf(v[4 * i + 1]) * inv,
-                           fp8_nan_if_inf(v[4 * i + 2]) * inv, fp8_nan_if_inf(v[4 * i + 3]) * inv);
+      words[i] = fp8_pack4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv, v[4 * i + 3] * inv);
     if (m0 + lane < a.M && (n0 & 127) == 0)
       a.out_scales[fp8_scale_offset(m0 + lane, n0 >> 7, (a.M + 127) / 128)] = static_cast<uint8_t>(byte);
     store_piece<1, false>(a, map, stg, words, m0, n0, tma, lane);
@@ -326,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < C::kAcc; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], CG == 2 ? 2 * kEpiWarps : kEpiWarps / 2);
+      mbar_init(&tempty[i], CG * kEpiWarps / C::kAcc);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&pairs[i], 2);
     fence_mbar_init();
@@ -344,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
@@ -368,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma2_load_2d(db, &tmB, fb, kb * 128, n0);
             if (sf) {
               tma2_load_2d(ds, &tmSA, fb, 0, (kb >> 2) * m_tiles + mt);
-              tma2_load_2d(ds + 512, &tmSB, fb, 0, (kb >> 2) * row_tiles_n + nt * 2);
+              tma2_load_2d(ds + 512, &tmSB, fb, 0, (kb >> 2) * row_tiles_n + nt * C::kSfBTiles);
             }
           } else {
             tma_load_2d(da, &tmA, &full[stage], kb * 128, mt * 128);
@@ -424,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int q = warp & 3, part = (warp - 4) >> 2;  // lane quarter, 64-column part of the tile
-    const int cols = (CG == 2 ? part : part & 1) * 64;
+    const int cols = (C::kAcc == 1 ? part : part & 1) * 64;
     uint8_t* stg = sEpi + (warp - 4) * kStageOut;
     uint8_t* tabs = sEpi + kEpiWarps * kStageOut;
     float* ctab = reinterpret_cast<float*>(tabs + (warp - 4) * kEpiTab);
@@ -435,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0;
     for (int t = unit; t < num_tiles; t += units, ++it) {
       const int acc = it % C::kAcc;
-      if (CG == 1 && acc != part >> 1) continue;  // the halves take alternate tiles
+      if (C::kAcc == 2 && acc != part >> 1) continue;  // the halves take alternate tiles
       const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
       const int m0 = mt * 128 + q * 32, n0 = nt * C::kBN + cols;
 #pragma unroll
@@ -466,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // whole 128-column blocks are in or out together, so both warps of a pair come here
       if (m0 < a.M && (n0 & ~127) < a.N &&
-          !epilogue64(a, &tmC, v, m0, n0, stg, ctab, other, pair, uses++ & 1, tma != 0, lane, status))
+          !epilogue64(a, &tmC, v, m0, n0, stg, ctab, other, pair, uses, tma != 0, lane, status))
         break;
     }
     if (lane == 0) bulk_wait_all();
@@ -541,18 +558,11 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                                 esz, a.M, a.N, a.ldo, 64 / esz, 32, CU_TENSOR_MAP_SWIZZLE_64B))
     return -2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long>(tiles, sm_count(dev) / CG) * CG));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_fp8_gemm<CG>, ta, tb, tsa, tsb, tc, a, tma, status) == cudaSuccess ? 0 : -4;
+  const unsigned grid = static_cast<unsigned>(std::min<long>(tiles, sm_count(dev) / CG) * CG);
+  return launch_pdl(k_fp8_gemm<CG>, dim3(grid), kThreads, C::kSmem, s, CG, ta, tb, tsa, tsb, tc, a, tma, status) ==
+                 cudaSuccess
+             ? 0
+             : -4;
 }
 
 }  // namespace
@@ -568,9 +578,20 @@ int check_linear_fp8(const Fp8Linear& a) {
 
 int linear_fp8(const Fp8Linear& a, int* status, cudaStream_t s) {
   if (a.M == 0) return 0;
-  const long pair_tiles = static_cast<long>((a.M + 255) / 256) * ((a.N + 255) / 256);
-  if (pair_tiles >= 74) return launch<2>(a, status, s);
-  return launch<1>(a, status, s);
+  // The tile shape with the shorter time: waves of tiles times a tile's time. A k-block brings
+  // 32 KB into an SM with either, which takes 800 to 900 cycles (measured at K = 4096 on one
+  // and on all SMs; the tensor work takes 256 or 512), and a pair's one accumulator waits
+  // another 1600 cycles a tile for the epilogue to read it. Measured at N = 4096, K = 1024
+  // and M = 1370, 2740, 5480: single CTAs 15, 25, 43 us, pairs 13, 23, 33; at N = 1024,
+  // K = 4096, M = 1370: 17 and 21.
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t sms = sm_count(dev), kb = (a.K + 127) / 128;
+  const int64_t tiles1 = (static_cast<int64_t>(a.M) + 127) / 128 * ((a.N + 127) / 128);
+  const int64_t tiles2 = (static_cast<int64_t>(a.M) + 255) / 256 * ((a.N + 255) / 256);
+  const int64_t time1 = (tiles1 + sms - 1) / sms * (kb * 800 + 300);
+  const int64_t time2 = (tiles2 + sms / 2 - 1) / (sms / 2) * (kb * 900 + 1600);
+  return time2 <= time1 ? launch<2>(a, status, s) : launch<1>(a, status, s);
 }
 
 }  // namespace da3b

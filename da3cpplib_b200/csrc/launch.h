@@ -1,0 +1,31 @@
+// Launches that may begin before the kernel ahead of them in the stream has ended
+// (programmatic dependent launch): the launch itself, and whatever a kernel does before
+// pdl_wait() (ptx.cuh), overlap that kernel's end. Every kernel launched so calls pdl_wait()
+// before its first access to global memory that another kernel may write or still read.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+namespace da3b {
+
+// cluster: CTAs a cluster along x (1: none).
+template <typename... Params, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
+                       unsigned cluster, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+}  // namespace da3b
