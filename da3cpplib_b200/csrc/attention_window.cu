@@ -316,7 +316,10 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         int st = 0;
         uint32_t par = 1;
         for (int i = 0; i <= n_all; ++i) {
-          if (!mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty)) break;
+          if (!mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty)) {
+            drain(kv_full, C::kRing, i, status);
+            break;
+          }
           uint8_t* dst = sKV + st * C::kStage;
           mbar_arrive_expect_tx(&kv_full[st], i == 0 || i == n_all ? C::kTile : C::kStage);
           if (i < n_all) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], col0(i));
@@ -809,7 +812,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (lane == 0) {
       for (int n = n_begin; n < n_end; ++n) {
         const int it = n - n_begin, st = it % C::kStages;
-        if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1u, status, kStatusTimeoutEmpty)) break;
+        if (!mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1u, status, kStatusTimeoutEmpty)) {
+          drain(full, C::kStages, it, status);
+          break;
+        }
         mbar_arrive_expect_tx(&full[st], 2 * C::kTile);
         uint8_t* k = smem + st * 2 * C::kTile;
         for (int c = 0; c < D / 64; ++c) tma_load_4d(k + c * 8192, &tmK, &full[st], c * 64, hk, key0(n), b);
@@ -1133,6 +1139,7 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
     if (reinterpret_cast<uintptr_t>(p) & 15) return -1;
   // 32-bit work counts inside
   if (static_cast<double>(nseq) * heads * q_len > 2147483647.0 * 8) return -1;
+  if (!writable_here(out)) return -104;
   int* st = device_status_word();
   if (!st) return -101;
   return attention_window(a, st, static_cast<cudaStream_t>(stream));

@@ -5,6 +5,8 @@
 // byte are written. Eight threads share a block of 128 columns (16 consecutive values
 // each), so the block's maximum takes three shuffles, the codes leave as one 16-byte
 // store a thread, and 32 threads together hold the four blocks of one scale word.
+#include <atomic>
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -191,7 +193,6 @@ bool bad_codes(const uint8_t* q, int ldq, const uint8_t* scales, int K) {
 template <typename T>
 int launch_quantize(const void* xv, int rows, int K, int ldx, uint8_t* q, int ldq, uint8_t* scales, cudaStream_t s) {
   const T* x = static_cast<const T*>(xv);
-  if (reinterpret_cast<uintptr_t>(x) % sizeof(T)) return -1;
   const dim3 grid((static_cast<unsigned>(rows) + 7) / 8, (static_cast<unsigned>(K) + 1023) / 1024);
   if (grid.y > 65535) return -1;
   cudaError_t e;
@@ -204,10 +205,35 @@ int launch_quantize(const void* xv, int rows, int K, int ldx, uint8_t* q, int ld
 
 }  // namespace
 
+bool writable_here(const void* p) {
+  typedef CUresult (*PFN_pointerAttribute)(void*, CUpointer_attribute, CUdeviceptr);
+  static std::atomic<PFN_pointerAttribute> known{nullptr};
+  PFN_pointerAttribute ask = known.load(std::memory_order_acquire);
+  if (!ask) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuPointerGetAttribute", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      return false;
+    ask = reinterpret_cast<PFN_pointerAttribute>(f);
+    known.store(ask, std::memory_order_release);
+  }
+  int dev = 0, at = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const CUdeviceptr d = reinterpret_cast<CUdeviceptr>(p);
+  if (ask(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, d) != CUDA_SUCCESS) return false;
+  if (at == dev) return true;
+  unsigned type = 0;  // pinned memory belongs to no device in particular
+  return ask(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, d) == CUDA_SUCCESS && type == CU_MEMORYTYPE_HOST;
+}
+
 int quantize_fp8(const void* x, int dtype, int rows, int K, int ldx, uint8_t* q, int ldq, uint8_t* scales,
                  cudaStream_t s) {
-  if (K <= 0 || ldx < K || bad_codes(q, ldq, scales, K)) return -1;
+  if (K <= 0 || K > kMostCount || rows > kMostCount || ldx < K || bad_codes(q, ldq, scales, K) || dtype < kF16 ||
+      dtype > kF32 || reinterpret_cast<uintptr_t>(x) % (dtype == kF32 ? 4 : 2))
+    return -1;
   if (rows == 0) return 0;
+  if (!writable_here(q) || !writable_here(scales)) return -104;
   switch (dtype) {
     case kF16: return launch_quantize<__half>(x, rows, K, ldx, q, ldq, scales, s);
     case kBF16: return launch_quantize<__nv_bfloat16>(x, rows, K, ldx, q, ldq, scales, s);
@@ -218,10 +244,11 @@ int quantize_fp8(const void* x, int dtype, int rows, int K, int ldx, uint8_t* q,
 
 int layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g, const float* b, float eps, uint8_t* q,
                   int ldq, uint8_t* scales, cudaStream_t s) {
-  if (K <= 0 || K > 16384 || ldx < K || bad_codes(q, ldq, scales, K) || !(eps >= 0.f)) return -1;
+  if (K <= 0 || K > 16384 || rows > kMostCount || ldx < K || bad_codes(q, ldq, scales, K) || !(eps >= 0.f)) return -1;
   if (reinterpret_cast<uintptr_t>(x) % 4 || reinterpret_cast<uintptr_t>(g) % 4 || reinterpret_cast<uintptr_t>(b) % 4)
     return -1;
   if (rows == 0) return 0;
+  if (!writable_here(q) || !writable_here(scales)) return -104;
   const bool vec = K % 16 == 0 && ldx % 8 == 0 && aligned32(x) && aligned32(g) && aligned32(b);
   const unsigned per_warp = static_cast<unsigned>((rows + 7) / 8), per_block = static_cast<unsigned>(rows);
   cudaError_t e;

@@ -179,7 +179,7 @@ __device__ __forceinline__ void store_piece(const Fp8Linear& a, const CUtensorMa
   if (tma) {
     if (lane == 0) bulk_wait_read<0>();  // the last piece has left the buffer
     __syncwarp();
-    tma = n0 + 64 / ESZ <= a.N || a.N * ESZ % 16 == 0;
+    tma = n0 + 64 / ESZ <= a.N || a.N % (16 / ESZ) == 0;
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -367,12 +367,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       int stage = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, loads = 0;
       bool ok = true;
       for (int t = unit; t < num_tiles && ok; t += units) {
         const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, status, kStatusTimeoutEmpty)) { ok = false; break; }
+          ++loads;
           const bool sf = (kb & 3) == 0;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * (C::kStageBytes + (sf ? C::kSfBytes : 0)));
           uint8_t* da = sA + stage * C::kABytes;
@@ -398,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
       }
+      if (!ok && rank == 0) drain(full, C::kStages, loads, status);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -568,7 +570,7 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
 }  // namespace
 
 int check_linear_fp8(const Fp8Linear& a) {
-  if (a.K <= 0 || a.N <= 0 || a.ldx < a.K || a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.ldo < a.N ||
+  if (a.K <= 0 || a.N <= 0 || a.M > kMostCount || a.N > kMostCount || a.K > kMostCount || a.ldx < a.K || a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.ldo < a.N ||
       !aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.xs, 16) || !aligned(a.ws, 16) ||
       !aligned(a.out, out_size(a.kind)) || !aligned(a.bias, 4) || !aligned(a.scale, 4))
     return -1;
@@ -577,7 +579,6 @@ int check_linear_fp8(const Fp8Linear& a) {
 }
 
 int linear_fp8(const Fp8Linear& a, int* status, cudaStream_t s) {
-  if (a.M == 0) return 0;
   // The tile shape with the shorter time: waves of tiles times a tile's time. A k-block brings
   // 32 KB into an SM with either, which takes 800 to 900 cycles (measured at K = 4096 on one
   // and on all SMs; the tensor work takes 256 or 512), and a pair's one accumulator waits
@@ -606,6 +607,8 @@ static int run_linear(const void* x, int M, int K, int ldx, const void* xs, cons
                        static_cast<const uint8_t*>(ws), M, N, K, ldx, ldw, bias, scale, act, kind, out, ldo,
                        static_cast<uint8_t*>(out_scales)};
   if (check_linear_fp8(a)) return -1;
+  if (M == 0) return 0;
+  if (!writable_here(out) || (out_scales && !writable_here(out_scales))) return -104;
   int* st = device_status_word();
   if (!st) return -101;
   return linear_fp8(a, st, static_cast<cudaStream_t>(stream));

@@ -28,4 +28,13 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, s
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Whether a buffer that a kernel is to write can be: memory of the current device, or
+// managed or pinned memory. Anything else (pageable host memory, another device's) would
+// fault in the kernel instead of failing here. Asked of the driver, which answers for one
+// attribute in a fraction of the time that the runtime's query of all of them takes.
+bool writable_here(const void* p);
+
+// Largest count of rows or columns: rounding up to a tile stays inside 32 bits.
+constexpr int kMostCount = 0x7fffff00;
+
 }  // namespace da3b

@@ -103,6 +103,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return __all_sync(0xffffffffu, ok);
 }
 
+// After a failed wait: gives the copies of the last loads into a ring (of `loads` issued so
+// far, one barrier phase each) the time of a few hundred tries to land, so that none writes
+// shared memory after the kernel has left.
+__device__ __forceinline__ void drain(uint64_t* full, int stages, uint32_t loads, int* status) {
+  for (uint32_t i = loads > static_cast<uint32_t>(stages) ? loads - stages : 0; i < loads; ++i)
+    mbar_wait(&full[i % stages], (i / stages) & 1, status, kStatusTimeoutFull);
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
   asm volatile(

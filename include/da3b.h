@@ -185,7 +185,7 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  *
  * A matrix [rows][K] (activations, or weights [N][K]) is held as e4m3 codes [rows][ld]
  * (ld bytes, ld >= K and a multiple of 16, base 16-byte aligned) and one scale for each
- * row and 128 columns: value = code * 2^(s - 127), s a byte. The scale bytes lie in
+ * row and 128 columns: value = code * 2^(s - 127), s a byte of at most 254. The scale bytes lie in
  * "scale tiles" (16-byte aligned, da3b_fp8_scale_bytes(rows, K) bytes): 512 bytes for each
  * 512 columns g and 128 rows t, in the order [g][t][32][4][4]; row 128 t + 32 c + l and
  * columns from 128 (4 g + j) on have theirs at [g][t][l][c][j]. Bytes of rows and columns
@@ -198,7 +198,8 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  *
  * Types: 0 f16, 1 bf16, 2 f32. All functions return 0 when launched, -100 for a null
  * pointer or a bad code or count, -1 for sizes, leading dimensions or alignments that are
- * not served, other negative values for launch errors. Calls with no rows do nothing.
+ * not served, -104 for an output that is not memory of the current device (or pinned or
+ * managed), other negative values for launch errors. Calls with no rows do nothing.
  * Nothing is allocated except the status word on a device's first call (make that one
  * outside of a stream capture); any number of calls may run at once. Pointers belong to
  * the current device, and outputs may not overlap inputs.

@@ -168,6 +168,15 @@ def test_negative_lengths_are_empty(lib):
     assert (o[0] == 7.0).all() and (o[1] == 0).all()
 
 
+def test_host_output_is_refused(lib):
+    q, k, v = make(1, 5, 9, 2, 2, 64, torch.float16, 6)
+    o = torch.zeros(q.numel() + 64, dtype=torch.float16)
+    h = (o.data_ptr() + 63) // 64 * 64
+    assert lib.da3b_attention_window(q.data_ptr(), s3(q), k.data_ptr(), s3(k), v.data_ptr(), s3(v), h, s3(q), 0, 1, 5, 9,
+                                     2, 2, 64, None, None, 3, 0, 1, 0.125, st()) == -104
+    assert (o == 0).all()
+
+
 def test_no_keys_at_all(lib):
     q, k, v = make(2, 33, 1, 2, 2, 64, torch.float16, 6)
     o = torch.full_like(q, 7.0)

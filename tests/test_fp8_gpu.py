@@ -279,6 +279,56 @@ def test_linear_quantised_output(lib, M, K, N, act):
     assert (q[:, N:] == 0x55).all()
 
 
+def test_host_outputs_are_refused(lib):
+    """An output in pageable host memory is refused before anything is launched."""
+    M, K, N = 4, 128, 32
+    (xq, xs, xv, wq, ws, wv), bias = make_linear(lib, M, K, N, 1)
+    x = torch.randn(M, K, device="cuda")
+    host = torch.zeros(4096, dtype=torch.uint8)
+    h = (host.data_ptr() + 63) // 64 * 64
+    args = (xq.data_ptr(), M, K, xq.stride(0), xs.data_ptr(), wq.data_ptr(), N, wq.stride(0), ws.data_ptr(), None)
+    assert lib.da3b_quantize_fp8(x.data_ptr(), 2, M, K, K, h, K, xs.data_ptr(), st()) == -104
+    assert lib.da3b_quantize_fp8(x.data_ptr(), 2, M, K, K, xq.data_ptr(), K, h, st()) == -104
+    assert lib.da3b_layernorm_fp8(x.data_ptr(), M, K, K, bias.data_ptr(), None, 1e-6, h, K, xs.data_ptr(), st()) == -104
+    assert lib.da3b_linear_fp8(*args, 0, h, 0, N, st()) == -104
+    assert lib.da3b_linear_fp8_q(*args, 0, xq.data_ptr(), N, h, st()) == -104
+    assert lib.da3b_linear_fp8_resid_f32(*args, None, h, N, st()) == -104
+    assert (host == 0).all()
+
+
+def test_linear_into_pinned_memory(lib):
+    M, K, N = 40, 256, 96
+    (xq, xs, xv, wq, ws, wv), bias = make_linear(lib, M, K, N, 1)
+    y = torch.zeros(M, N).pin_memory()
+    d = torch.zeros(M, N, device="cuda")
+    for o in (y, d):
+        assert lib.da3b_linear_fp8(xq.data_ptr(), M, K, xq.stride(0), xs.data_ptr(), wq.data_ptr(), N, wq.stride(0),
+                                   ws.data_ptr(), bias.data_ptr(), 0, o.data_ptr(), 2, N, st()) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, d.cpu())
+
+
+def test_quantised_output_with_infinities(lib):
+    """A product that overflows (a scale of 2^120 against one of 2^20) gives infinities and NaN:
+    NaN codes, and the scale of the block's finite values; other rows are as ever."""
+    M, K, N = 150, 256, 300
+    (xq, xs, xv, wq, ws, wv), bias = make_linear(lib, M, K, N, 6)
+    b, wb = bytes_of(xs, M, K).clone(), bytes_of(ws, N, K).clone()
+    b[9], wb[200:] = 247, 160
+    xs2, ws2 = tiles_of(b, K), tiles_of(wb, K)
+    q = torch.empty(M, up(N, 16), dtype=torch.uint8, device="cuda")
+    s = torch.empty(lib.da3b_fp8_scale_bytes(M, N), dtype=torch.uint8, device="cuda")
+    y = torch.empty(M, N, device="cuda")
+    args = (xq.data_ptr(), M, K, xq.stride(0), xs2.data_ptr(), wq.data_ptr(), N, wq.stride(0), ws2.data_ptr(), bias.data_ptr(), 0)
+    assert lib.da3b_linear_fp8_q(*args, q.data_ptr(), up(N, 16), s.data_ptr(), st()) == 0
+    assert lib.da3b_linear_fp8(*args, y.data_ptr(), 2, N, st()) == 0
+    assert not torch.isfinite(y[9, 200:]).all() and torch.isfinite(y[:9]).all()
+    codes, want = plain_quant(y)
+    nan = (codes & 0x7F) == 0x7F
+    assert nan.any() and torch.equal((q[:, :N] & 0x7F) == 0x7F, nan)
+    assert torch.equal(q[:, :N][~nan], codes[~nan]) and torch.equal(bytes_of(s, M, N), want)
+
+
 def test_linear_nan_stays_in_its_row(lib):
     """A NaN activation makes its row NaN and no other; rows past M and columns past K hold
     NaN codes and NaN scales already (make_linear)."""

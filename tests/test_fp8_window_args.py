@@ -24,7 +24,7 @@ QUANT = dict(x=P, dtype=0, rows=4, K=100, ldx=100, q=P, ldq=112, scales=P)
     (dict(x=None), -100), (dict(q=None), -100), (dict(scales=None), -100), (dict(rows=-1), -100),
     (dict(K=0), -1), (dict(K=-5), -1), (dict(ldx=99), -1), (dict(ldq=100), -1), (dict(ldq=96), -1),
     (dict(q=P + 8), -1), (dict(scales=P + 4), -1), (dict(dtype=3), -1), (dict(dtype=-1), -1), (dict(x=P + 1), -1),
-    (dict(rows=0), 0),
+    (dict(rows=0), 0), (dict(rows=(1 << 31) - 1), -1), (dict(K=(1 << 31) - 1, ldx=(1 << 31) - 1, ldq=(1 << 31) - 16), -1),
 ])
 def test_quantize_refusals(lib, change, rc):
     a = {**QUANT, **change}
@@ -49,7 +49,8 @@ COMMON = [
     (dict(x=None), -100), (dict(xs=None), -100), (dict(w=None), -100), (dict(ws=None), -100), (dict(out=None), -100),
     (dict(M=-1), -100), (dict(K=0), -1), (dict(N=0), -1), (dict(ldx=96), -1),
     (dict(ldx=100), -1), (dict(ldw=104), -1), (dict(x=P + 8), -1), (dict(w=P + 1), -1), (dict(xs=P + 4), -1),
-    (dict(ws=P + 8), -1), (dict(bias=P + 2), -1), (dict(ldo=29), -1),
+    (dict(ws=P + 8), -1), (dict(bias=P + 2), -1), (dict(ldo=29), -1), (dict(M=0), 0), (dict(M=(1 << 31) - 1), -1),
+    (dict(N=(1 << 31) - 1, ldo=(1 << 31) - 1), -1),
 ]
 
 
