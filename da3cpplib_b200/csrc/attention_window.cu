@@ -50,8 +50,8 @@ constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the r
 
 template <int D>
 struct WinCfg {
-  static constexpr int kNT = D == 64 ? 3 : 2;  // query tiles
-  static constexpr int kKT = 64;               // keys a tile
+  static constexpr int kNT = D == 64 ? 3 : 2;    // query tiles
+  static constexpr int kKT = D == 64 ? 64 : 80;  // keys a tile
   static constexpr int kThreads = 128 + 128 * kNT;
   // registers move from the first warpgroup to the softmax's (setmaxnreg); the split may not
   // exceed what the launch holds
@@ -106,7 +106,8 @@ __device__ __forceinline__ float2 exp2_cubic(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// N columns of this thread's lane of tensor memory, there after tmem_wait_ld and landed.
+// N columns (a multiple of 16) of this thread's lane of tensor memory, there after
+// tmem_wait_ld and landed.
 template <int N>
 __device__ __forceinline__ void load_cols(uint32_t taddr, float (&s)[N]) {
 #pragma unroll
@@ -123,7 +124,33 @@ __device__ __forceinline__ void load_cols(uint32_t taddr, float (&s)[N]) {
           "=f"(s[32 * i + 23]), "=f"(s[32 * i + 24]), "=f"(s[32 * i + 25]), "=f"(s[32 * i + 26]), "=f"(s[32 *
           i + 27]), "=f"(s[32 * i + 28]), "=f"(s[32 * i + 29]), "=f"(s[32 * i + 30]), "=f"(s[32 * i + 31])
         : "r"(taddr + 32 * i));
+  if constexpr (N % 32 != 0)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(s[N - 16 + 0]), "=f"(s[N - 16 + 1]), "=f"(s[N - 16 + 2]), "=f"(s[N - 16 + 3]), "=f"(s[N - 16 +
+          4]), "=f"(s[N - 16 + 5]), "=f"(s[N - 16 + 6]), "=f"(s[N - 16 + 7]), "=f"(s[N - 16 + 8]), "=f"(s[N -
+          16 + 9]), "=f"(s[N - 16 + 10]), "=f"(s[N - 16 + 11]), "=f"(s[N - 16 + 12]), "=f"(s[N - 16 + 13]),
+          "=f"(s[N - 16 + 14]), "=f"(s[N - 16 + 15])
+        : "r"(taddr + N - 16));
 }
+// N words (32, 64, or 32 and 8 more) into this thread's lane, there after tmem_wait_st.
+template <int N>
+__device__ __forceinline__ void store_words(uint32_t taddr, const uint32_t (&w)[N]) {
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) {
+    uint32_t x[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = w[32 * i + j];
+    tmem_st32(taddr + 32 * i, x);
+  }
+  if constexpr (N % 32 != 0)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr + N - 8),
+                 "r"(w[N - 8]), "r"(w[N - 7]), "r"(w[N - 6]), "r"(w[N - 5]), "r"(w[N - 4]), "r"(w[N - 3]), "r"(w[N - 2]),
+                 "r"(w[N - 1])
+                 : "memory");
+}
+
 // The lowest n bits (none for n <= 0, all for n >= 32). Masks are taken from such words:
 // compared column by column against a row's bounds, a cut tile took thousands of cycles.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
@@ -450,10 +477,10 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
         const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
-        for (int w = 0; w < KT / 32; ++w) {
+        for (int w = 0; w < (KT + 31) / 32; ++w) {
           const uint32_t bits = below(x1 + 1 - 32 * w) & (~below(x0 - 32 * w) | below(x2 - 32 * w));
 #pragma unroll
-          for (int i = 0; i < 32; ++i) s[32 * w + i] = bits >> i & 1u ? s[32 * w + i] : -INFINITY;
+          for (int i = 0; i < 32 && 32 * w + i < KT; ++i) s[32 * w + i] = bits >> i & 1u ? s[32 * w + i] : -INFINITY;
         }
       }
       float m8[8];
@@ -497,7 +524,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         }
       }
       l += s2.x + s2.y;
-      tmem_st32(tP, pk);
+      store_words<KT / 2>(tP, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -689,7 +716,7 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   // the times measured (ns a key tile for 1, 2, .. query tiles). A view of 1297 tokens and 16
   // heads over 7800 keys: 48 items of four tiles leave 100 SMs idle unsplit, and two thirds
   // of them in two; 64 items of three tiles in two fill 128.
-  constexpr int64_t kTileNs[2][3] = {{750, 1050, 1250}, {780, 1070, 0}};
+  constexpr int64_t kTileNs[2][3] = {{750, 1050, 1250}, {980, 1350, 0}};
   constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
   int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
