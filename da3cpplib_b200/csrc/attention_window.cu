@@ -51,17 +51,17 @@ constexpr float kRaise = 8.0f;          // log2 by which a tile may exceed the r
 template <int D>
 struct WinCfg {
   static constexpr int kNT = D == 64 ? 3 : 2;    // query tiles
-  static constexpr int kKT = D == 64 ? 64 : 80;  // keys a tile
+  static constexpr int kKT = D == 64 ? 48 : 64;  // keys a tile
   static constexpr int kThreads = 128 + 128 * kNT;
   // registers move from the first warpgroup to the softmax's (setmaxnreg); the split may not
   // exceed what the launch holds
-  static constexpr int kRegsLaunch = D == 64 ? 128 : 168, kRegsCtl = D == 64 ? 80 : 72, kRegsSoft = D == 64 ? 144 : 216;
+  static constexpr int kRegsLaunch = kNT == 3 ? 128 : 168, kRegsCtl = kNT == 3 ? 80 : 72, kRegsSoft = kNT == 3 ? 144 : 216;
   static_assert(128 * kRegsCtl + 128 * kNT * kRegsSoft <= kThreads * kRegsLaunch, "register split");
   static constexpr int kQTile = 128 * D * 2, kTile = kKT * D * 2;  // bytes of a Q and of a K or V tile
-  static constexpr int kRing = D == 64 ? 8 : 4;     // stages of a V tile and a K tile
-  static constexpr int kStage = 2 * kTile, kRingBytes = kRing * kStage;
-  static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 256;
-  static constexpr uint32_t kColP = kNT * kKT, kColO = kColP + kNT * kKT / 2;  // behind S_t
+  static constexpr int kStage = 2 * kTile;          // a V tile and a K tile
+  static constexpr int kRing = D == 64 ? 10 : 5, kRingBytes = kRing * kStage;
+  static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 512;
+  static constexpr uint32_t kColO = 2 * kNT * kKT;  // behind two S_t each
   static_assert(kColO + kNT * D <= 512, "tensor memory");
   // a CTA's share of a split item: O rows, then (m, l), over the Q tiles and the ring
   static constexpr int kShareO = kNT * 128 * D * 4;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void load_cols(uint32_t taddr, float (&s)[N]) {
           "=f"(s[N - 16 + 14]), "=f"(s[N - 16 + 15])
         : "r"(taddr + N - 16));
 }
-// N words (32, 64, or 32 and 8 more) into this thread's lane, there after tmem_wait_st.
+// N words (a multiple of 8) into this thread's lane, there after tmem_wait_st.
 template <int N>
 __device__ __forceinline__ void store_words(uint32_t taddr, const uint32_t (&w)[N]) {
 #pragma unroll
@@ -144,7 +144,14 @@ __device__ __forceinline__ void store_words(uint32_t taddr, const uint32_t (&w)[
     for (int j = 0; j < 32; ++j) x[j] = w[32 * i + j];
     tmem_st32(taddr + 32 * i, x);
   }
-  if constexpr (N % 32 != 0)
+  constexpr int r = N / 32 * 32;
+  if constexpr (N % 32 >= 16) {
+    uint32_t x[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = w[r + j];
+    tmem_st16(taddr + r, x);
+  }
+  if constexpr (N % 16 != 0)
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr + N - 8),
                  "r"(w[N - 8]), "r"(w[N - 7]), "r"(w[N - 6]), "r"(w[N - 5]), "r"(w[N - 4]), "r"(w[N - 3]), "r"(w[N - 2]),
                  "r"(w[N - 1])
@@ -260,16 +267,16 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                       // [NT]
-  // the ring: load i brings V of tile i - 1 and K of tile i (there is no tile -1 or n_all)
+  // the ring: load i brings V of tile i - 2 and K of tile i, where there are such tiles
   uint8_t* sKV = sQ + NT * C::kQTile;       // [kRing] V, K
   uint64_t* q_full = reinterpret_cast<uint64_t*>(sKV + C::kRingBytes);
   uint64_t* kv_full = q_full + 1;           // [kRing]
   uint64_t* kv_empty = kv_full + C::kRing;  // [kRing] (every issuing warp)
-  uint64_t* s_full = kv_empty + C::kRing;   // [NT] S_t complete
-  uint64_t* s_free = s_full + NT;           // [NT] S_t in registers (4 warps)
-  uint64_t* p_ready = s_free + NT;          // [NT] P_t written, O_t rescaled, V rows zeroed (4 warps)
-  uint64_t* pv_done = p_ready + NT;         // [NT] P_t V complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NT);
+  // one barrier for the even and one for the odd ones of the tiles that query tile t sees:
+  uint64_t* s_full = kv_empty + C::kRing;   // [NT][2] S_t complete (and the product two before)
+  uint64_t* p_ready = s_full + 2 * NT;      // [NT][2] P_t written, O_t rescaled, V rows zeroed (4 warps)
+  uint64_t* pv_done = p_ready + 2 * NT;     // [NT][2] P_t V complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2 * NT);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a cluster of nsplit CTAs shares an item's key tiles; a sequence's last tokens come first:
@@ -304,9 +311,8 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], NT);
     }
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < 2 * NT; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_free[t], 4);
       mbar_init(&p_ready[t], 4);
       mbar_init(&pv_done[t], 1);
     }
@@ -342,15 +348,16 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         };
         int st = 0;
         uint32_t par = 1;
-        for (int i = 0; i <= n_all; ++i) {
+        for (int i = 0; i < n_all + 2; ++i) {
           if (!mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty)) {
             drain(kv_full, C::kRing, i, status);
             break;
           }
           uint8_t* dst = sKV + st * C::kStage;
-          mbar_arrive_expect_tx(&kv_full[st], i == 0 || i == n_all ? C::kTile : C::kStage);
-          if (i < n_all) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], col0(i));
-          if (i > 0) load_tile(dst, tmV, tmV8, &kv_full[st], col0(i - 1));
+          const bool k = i < n_all, v = i >= 2;
+          mbar_arrive_expect_tx(&kv_full[st], (k ? C::kTile : 0) + (v ? C::kTile : 0));
+          if (k) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], col0(i));
+          if (v) load_tile(dst, tmV, tmV8, &kv_full[st], col0(i - 2));
           if (++st == C::kRing) { st = 0; par ^= 1u; }
         }
       }
@@ -367,64 +374,51 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       const int t = warp - 1;
       const uint64_t qd = umma_desc_sw128(smem_u32(sQ) + t * C::kQTile);
       const uint64_t vd0 = desc_mn_sw128(smem_u32(sKV), KT * 128), kd0 = umma_desc_sw128(smem_u32(sKV) + C::kTile);
-      const uint32_t tS = tmem + t * KT, tP = tmem + C::kColP + t * (KT / 2), tO = tmem + C::kColO + t * D;
+      const uint32_t tS = tmem + 2 * t * KT, tO = tmem + C::kColO + t * D;
       const Seen<KT> see(span(t), a.sinks);
+      int ns = 0, np = 0;  // S and P V products issued
       auto issue_s = [&](int st) {
         const uint64_t kd = kd0 + st * (C::kStage >> 4);
+        const uint32_t d = tS + (ns & 1) * KT;
         if (one) {
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tS, qd + c * 1024 + 2 * kk, kd + c * (KT * 8) + 2 * kk, id_s, (c > 0 || kk > 0) ? 1u : 0u);
-          umma_commit(&s_full[t]);
+              umma_f16(d, qd + c * 1024 + 2 * kk, kd + c * (KT * 8) + 2 * kk, id_s, (c > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&s_full[2 * t + (ns & 1)]);
         }
         __syncwarp();
+        ++ns;
       };
-      bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull) &&
-                mbar_wait_warp(&kv_full[0], 0, status, kStatusTimeoutFull);
-      bool now = see.some(n0);
-      int ns = 0, np = 0;  // S and P V products issued
-      if (ok) {
-        tc_fence_after();
-        if (now) {
-          issue_s(0);
-          ++ns;
-        }
-        if (one) umma_commit(&kv_empty[0]);
-        __syncwarp();
-      }
-      int st = 1 % C::kRing;
-      uint32_t par = C::kRing == 1;
-      for (int n = 0; n < n_all && ok; ++n) {
-        const bool next = n + 1 < n_all && see.some(n0 + n + 1);
+      bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull);
+      int st = 0;
+      uint32_t par = 0;
+      for (int i = 0; i < n_all + 2 && ok; ++i) {
         ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
-        if (ok && next) {
-          if (ns > 0) ok = mbar_wait_warp(&s_free[t], (ns - 1) & 1, status, kStatusTimeoutAccumFree);
-          if (ok) {
-            tc_fence_after();
-            issue_s(st);
-            ++ns;
-          }
-        }
-        if (ok && now) {
-          ok = mbar_wait_warp(&p_ready[t], np & 1, status, kStatusTimeoutFull);
+        if (ok && i >= 2 && see.some(n0 + i - 2)) {
+          ok = mbar_wait_warp(&p_ready[2 * t + (np & 1)], (np >> 1) & 1, status, kStatusTimeoutFull);
           if (ok) {
             tc_fence_after();
             const uint64_t vd = vd0 + st * (C::kStage >> 4);
+            const uint32_t p = tS + (np & 1) * KT;
             if (one) {
 #pragma unroll
               for (int kk = 0; kk < KT / 16; ++kk)
-                umma_f16_tmem_a(tO, tP + 8 * kk, vd + 128 * kk, id_o, (np > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&pv_done[t]);
+                umma_f16_tmem_a(tO, p + 8 * kk, vd + 128 * kk, id_o, (np > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&pv_done[2 * t + (np & 1)]);
             }
             __syncwarp();
             ++np;
           }
         }
+        // behind the product that read the P_t in its place
+        if (ok && i < n_all && see.some(n0 + i)) {
+          tc_fence_after();
+          issue_s(st);
+        }
         if (ok && one) umma_commit(&kv_empty[st]);
         __syncwarp();
-        now = next;
         if (++st == C::kRing) { st = 0; par ^= 1u; }
       }
     }
@@ -438,12 +432,12 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;
     const int plain0 = max(see.whole0, fix1 + 1), plain1 = min(min(see.whole1, see.last), fix2 < 0 ? see.whole1 : fix2 - 1);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
-    const uint32_t tS = tmem + t * KT + lanes, tP = tmem + C::kColP + t * (KT / 2) + lanes, tO = tmem + C::kColO + t * D + lanes;
+    const uint32_t tS0 = tmem + 2 * t * KT + lanes, tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
     const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
     const int row_hi = min(kl - 1, p + a.right) + cols.shift(), row_lo = p - a.left + cols.shift();  // columns
     float m = -INFINITY, l = 0.f;
-    int cnt = 0, st = 0;
+    int cnt = 0, st = 1;
     uint32_t par = 0;
     bool ok = true;
     for (int n = 0; n < n_all && ok; ++n) {
@@ -451,7 +445,8 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       const bool plain = n0 + n >= plain0 && n0 + n <= plain1;
       if (!plain && !see.some(n0 + n)) continue;
       const int v0 = col0(n);
-      ok = mbar_wait_warp(&s_full[t], cnt & 1, status, kStatusTimeoutAccum);
+      const uint32_t tS = tS0 + (cnt & 1) * KT;  // S_t, then P_t
+      ok = mbar_wait_warp(&s_full[2 * t + (cnt & 1)], (cnt >> 1) & 1, status, kStatusTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
       float s[KT];
@@ -470,9 +465,6 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       }
       tmem_wait_ld();
       landed<KT>(s);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[t]);
       if (!plain && !see.whole(n0 + n)) {
         // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
         const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
@@ -505,34 +497,33 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         pk[i] = pack2<BF16>(e.x, e.y);
       }
       const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-      // behind the exponentials: P of the last tile has been read, and O_t is complete
-      if (cnt > 0) {
-        ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+      // O_t is rescaled behind the last tile's product (the one before that is complete: S_t of
+      // this tile was issued after it, so no phase of the barrier is missed)
+      if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
+        ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
         if (!ok) break;
         tc_fence_after();
-        if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll 1
-          for (int i = 0; i < D; i += 16) {
-            uint32_t w[16];
-            tmem_ld16(tO + i, w);
-            tmem_wait_ld();
+        for (int i = 0; i < D; i += 16) {
+          uint32_t w[16];
+          tmem_ld16(tO + i, w);
+          tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
-            tmem_st16(tO + i, w);
-          }
-          l *= alpha;
+          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+          tmem_st16(tO + i, w);
         }
+        l *= alpha;
       }
       l += s2.x + s2.y;
-      store_words<KT / 2>(tP, pk);
+      store_words<KT / 2>(tS, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
+      if (lane == 0) mbar_arrive(&p_ready[2 * t + (cnt & 1)]);
       ++cnt;
     }
     if (ok && cnt > 0) {
-      ok = mbar_wait_warp(&pv_done[t], (cnt - 1) & 1, status, kStatusTimeoutAccum);
+      ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
       tc_fence_after();
     }
     ok = __all_sync(0xffffffffu, ok);
@@ -716,7 +707,7 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   // the times measured (ns a key tile for 1, 2, .. query tiles). A view of 1297 tokens and 16
   // heads over 7800 keys: 48 items of four tiles leave 100 SMs idle unsplit, and two thirds
   // of them in two; 64 items of three tiles in two fill 128.
-  constexpr int64_t kTileNs[2][3] = {{750, 1050, 1250}, {980, 1350, 0}};
+  constexpr int64_t kTileNs[2][3] = {{500, 700, 850}, {700, 950, 0}};
   constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
   int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
