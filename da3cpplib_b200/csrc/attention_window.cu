@@ -24,23 +24,29 @@ namespace da3b {
 namespace {
 
 // ------------------------------------------------------------------ many queries
-// Several tiles of 128 query rows a CTA (one CTA per SM) share every key tile: three at
-// head_dim 64, two at 128. A query row is one (token, head): g query heads that share a key
-// head lie side by side, 128 / g tokens a tile, so that shared heads read their keys once
-// and a tile spans few positions (a window's ends are masked work).
-//   warp 0     TMA: the Q tiles, then the key tiles that some row sees, V of a tile together
-//              with K of the next in a ring ([keys][64 dims] boxes, 128B swizzle);
-//   warps 1..  one a query tile: S_t = Q_t K^T of the next key tile as soon as the last
-//              scores are in registers, and O_t += P_t V once P_t is there (P_t from tensor
-//              memory; V is read as it lies, its dims contiguous: an MN-major operand);
+// Several tiles of 128 query rows a CTA (one CTA per SM) share every key tile: three with key
+// tiles of 48 at head_dim 64, two with key tiles of 64 at 128. A query row is one (token,
+// head): g query heads that share a key head lie side by side, 128 / g tokens a tile, so that
+// shared heads read their keys once and a tile spans few positions (a window's ends are
+// masked work).
+//   warp 0     TMA: the Q tiles, then the key tiles that some row sees, K of a tile together
+//              with V of the tile two before in a ring ([keys][64 dims] boxes, 128B swizzle);
+//   warps 1..  one a query tile: O_t += P_t V (P_t from tensor memory; V is read as it lies,
+//              its dims contiguous: an MN-major operand), then S_t = Q_t K^T two tiles on;
 //   warps 4..  softmax, four a query tile: thread = row (its TMEM lane), the row's scores in
 //              registers, one pass; P back to tensor memory.
-// What a query tile waits for is hidden twice: its next scores are made while it takes its
-// exponentials (S_t and P_t have columns of their own: with P_t over S_t the two products
-// followed the softmax, a turn of 1880 cycles for 64 keys), and the other tiles fill the
-// rest. Each tile has an issuing warp of its own because few products wait in the tensor
-// pipe's queue: one warp's waits (about 100 cycles each, also where nothing is to be waited
-// for) leave the pipe idle.
+// Tensor memory holds two S_t for each query tile, taken in turn, and P_t lies over its S_t:
+// the scores of the next key tile are there when a softmax is done, and one barrier each way
+// is enough. What bounds it is that softmax, a chain of its own: 16384 keys, 9 x 16 CTAs, take
+// 942 ns a step of 48 keys at head_dim 64 (1064 ns a step of 64 at 128), 858 (904) without the
+// products, 660 (968) without the exponentials, and 540 (536) without both, which is what
+// the waits, the trip from and to tensor memory and the maximum take. Several query tiles
+// fill each other's waits; tensor memory has no room for more of them. Full attention of 4096
+// tokens runs at 694 and 1082 TFLOP/s. Taken otherwise: P_t over a single S_t (746 us against
+// 793 in that measure with four query tiles, but 114 against 86 for a new view of 1297
+// tokens, whose items then fill 96 SMs), S_t and P_t in columns of their own (802 us, 90), two
+// softmax threads a row (1057 us), one issuing warp for all query tiles (its waits, about
+// 100 cycles each, leave the tensor pipe idle).
 // The maximum of a row is raised only when a tile exceeds it by more than 2^8; O_t is then
 // rescaled in tensor memory. Sums are f32 of the unrounded probabilities.
 // Masks are applied to the tiles that a window's end, the sinks' end or the last key cuts.
@@ -704,10 +710,10 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   }
   // Query tiles a CTA, and a split of its key tiles over a cluster: whatever makes the call
   // shortest. CTAs run one an SM, so a call takes its waves of CTAs times a CTA's time, with
-  // the times measured (ns a key tile for 1, 2, .. query tiles). A view of 1297 tokens and 16
-  // heads over 7800 keys: 48 items of four tiles leave 100 SMs idle unsplit, and two thirds
-  // of them in two; 64 items of three tiles in two fill 128.
-  constexpr int64_t kTileNs[2][3] = {{500, 700, 850}, {700, 950, 0}};
+  // the times measured (ns a key tile for 1, 2, .. query tiles; setup and joining about 4 and
+  // 5 us). A view of 1297 tokens and 16 heads over 7800 keys: 64 items of three query tiles,
+  // each split in two, take 85 us; unsplit 149, 96 unsplit items of two query tiles 133.
+  constexpr int64_t kTileNs[2][3] = {{560, 770, 865}, {720, 1000, 0}};
   constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
   int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
