@@ -117,9 +117,19 @@ int* device_status_word() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   std::lock_guard<std::mutex> lk(g_status_mu);
   if (!g_status_words[dev]) {
+    // The first call on a device may be one that a stream captures: neither the allocation
+    // nor the clearing (on a stream of its own) is part of that capture or ends it.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
     int* p = nullptr;
-    if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-    if (cudaMemset(p, 0, sizeof(int)) != cudaSuccess) return nullptr;
+    cudaStream_t s = nullptr;
+    bool ok = cudaMalloc(&p, sizeof(int)) == cudaSuccess &&
+              cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
+              cudaMemsetAsync(p, 0, sizeof(int), s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess;
+    if (s) cudaStreamDestroy(s);
+    if (!ok && p) cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
     g_status_words[dev] = p;
   }
   return g_status_words[dev];

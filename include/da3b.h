@@ -200,9 +200,9 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  * pointer or a bad code or count, -1 for sizes, leading dimensions or alignments that are
  * not served, -104 for an output that is not memory of the current device (or pinned or
  * managed), other negative values for launch errors. Calls with no rows do nothing.
- * Nothing is allocated except the status word on a device's first call (make that one
- * outside of a stream capture); any number of calls may run at once. Pointers belong to
- * the current device, and outputs may not overlap inputs.
+ * Nothing is allocated except the status word on a device's first call; any number of
+ * calls may run at once, and a stream may capture any of them. Pointers belong to the
+ * current device, and outputs may not overlap inputs.
  * ---------------------------------------------------------------------- */
 DA3B_API size_t da3b_fp8_scale_bytes(int rows, int K);
 
