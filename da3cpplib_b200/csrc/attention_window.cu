@@ -660,10 +660,8 @@ int clusters_at_once(int ns, int dev) {
   using C = WinCfg<D>;
   static std::atomic<int> known[64][9];
   int n = known[dev & 63][ns].load(std::memory_order_relaxed);
-  if (n == 0 && ns == 1) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    known[dev & 63][ns].store(n, std::memory_order_relaxed);
-  } else if (n == 0) {
+  if (ns == 1) return sm_count(dev);
+  if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(ns));
     cfg.blockDim = dim3(C::kThreads);
@@ -1130,12 +1128,12 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
                                    int dtype, int nseq, int q_len, int k_len, int heads, int kv_heads, int head_dim,
                                    const int* q_lens, const int* k_lens, int left, int right, int sinks, float scale,
                                    void* stream) {
-  if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return -100;
   if ((dtype != 0 && dtype != 1) || nseq < 0 || q_len < 0 || k_len < 0 || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads || (head_dim != 64 && head_dim != 128) || sinks < 0 || !(scale >= 0.f) || isinf(scale))
     return -100;
   if (q_len > kWindowAll || k_len > kWindowAll) return -1;
   if (nseq == 0 || q_len == 0) return 0;
+  if (!q || !out || !q_strides || !k_strides || !v_strides || !out_strides || (k_len > 0 && (!k || !v))) return -100;
   AttnWindow a;
   a.q = q;
   a.k = k;
@@ -1155,8 +1153,8 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
   a.sinks = sinks;
   a.scale = fmaxf(scale, 1e-30f);  // at 0 a masked score (-inf) times it would be NaN
   if (!take_strides(q_strides, nseq, q_len, heads, head_dim, &a.qs) ||
-      !take_strides(k_strides, nseq, k_len, kv_heads, head_dim, &a.ks) ||
-      !take_strides(v_strides, nseq, k_len, kv_heads, head_dim, &a.vs) ||
+      (k_len > 0 && (!take_strides(k_strides, nseq, k_len, kv_heads, head_dim, &a.ks) ||
+                     !take_strides(v_strides, nseq, k_len, kv_heads, head_dim, &a.vs))) ||
       !take_strides(out_strides, nseq, q_len, heads, head_dim, &a.os))
     return -1;
   for (const void* p : {q, k, v, static_cast<const void*>(out)})

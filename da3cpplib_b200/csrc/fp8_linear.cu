@@ -19,9 +19,16 @@
 //              bias, activation, quantisation -> 64-byte row pieces in a swizzled staging
 //              buffer, stored (or, onto the residual, added) by TMA: the load-store unit,
 //              73 % busy with the pieces' reads and stores when the warps made them, only
-//              writes the buffer. Four
-//              warps an SM sub-partition hide each other's latencies: with eight warps of
-//              128 columns, M = 87680, K = 1024, N = 4096 with GELU took 528-580 us.
+//              writes the buffer. Four warps an SM sub-partition hide each other's
+//              latencies: M = 87680, K = 1024, N = 4096 with GELU to f16 takes 400-430 us,
+//              eight warps of 128 columns took 528-580.
+//
+// Bound: the MMAs (K = 1024: 4096 cycles a 256 x 256 tile at the full rate) and, one
+// accumulator to a CTA pair, the handover between them and the epilogue's reads. That shape
+// takes 343 us without an activation (2.14 PFLOP/s; the chip's power, at 1.5-1.6 GHz);
+// M = 21920 takes 87, K = 4096, N = 1024 79 (2.33 PFLOP/s). With GELU the epilogue's own
+// instructions (17 a value, two of them MUFU) are as long as the MMAs: 103 us at M = 21920,
+// 114 quantised. A ring of five stages: four and six measured the same.
 // Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
 #include <algorithm>
 #include <atomic>
@@ -123,7 +130,8 @@ __device__ __forceinline__ void copy_sf(uint32_t tmem, uint32_t saddr) {
 // 6.8e-8; beyond 6, v^2 is held at 36 and Phi is 0 or 1 to 1e-9. Ten multiply-adds and two
 // MUFU operations a value; the four pairs run side by side, because a chain of about
 // fifteen dependent operations a value otherwise leaves the pipes idle (the M = 87680,
-// K = 1024, N = 4096 product with GELU took 723 us with one chain at a time).
+// K = 1024, N = 4096 product with GELU: 723 us with one chain at a time, 400-430 so). One
+// reciprocal for two values (of the product of their denominators) was no faster: 417-430.
 __device__ __forceinline__ void gelu8(float* v) {
   float2 x[4], q[4];
   const float2 one = make_float2(1.f, 1.f);
@@ -518,16 +526,6 @@ int map_scales(CUtensorMap* m, const uint8_t* p, int rows, int K, int tiles) {
                             CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-int sm_count(int dev) {
-  static std::atomic<int> counts[64];
-  int n = counts[dev & 63].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    counts[dev & 63].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 template <int CG>
 int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
   using C = Cfg<CG>;
@@ -602,7 +600,7 @@ using namespace da3b;
 static int run_linear(const void* x, int M, int K, int ldx, const void* xs, const void* w, int N, int ldw,
                       const void* ws, const float* bias, const float* scale, int act, int kind, void* out, int ldo,
                       void* out_scales, void* stream) {
-  if (!x || !xs || !w || !ws || !out || M < 0 || act < 0 || act > 3) return -100;
+  if (!w || !ws || M < 0 || (M > 0 && (!x || !xs || !out)) || act < 0 || act > 3) return -100;
   const Fp8Linear a = {static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w),
                        static_cast<const uint8_t*>(ws), M, N, K, ldx, ldw, bias, scale, act, kind, out, ldo,
                        static_cast<uint8_t*>(out_scales)};
@@ -627,7 +625,7 @@ DA3B_API int da3b_linear_fp8(const void* x, int M, int K, int ldx, const void* x
 DA3B_API int da3b_linear_fp8_q(const void* x, int M, int K, int ldx, const void* x_scales, const void* w, int N,
                                int ldw, const void* w_scales, const float* bias, int act, void* out_q, int ldo,
                                void* out_scales, void* stream) {
-  if (!out_scales) return -100;
+  if (!out_scales && M > 0) return -100;
   return run_linear(x, M, K, ldx, x_scales, w, N, ldw, w_scales, bias, nullptr, act, kFp8OutQ, out_q, ldo, out_scales,
                     stream);
 }

@@ -34,6 +34,9 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, s
 // attribute in a fraction of the time that the runtime's query of all of them takes.
 bool writable_here(const void* p);
 
+// Multiprocessors of a device (asked once).
+int sm_count(int dev);
+
 // Largest count of rows or columns: rounding up to a tile stays inside 32 bits.
 constexpr int kMostCount = 0x7fffff00;
 

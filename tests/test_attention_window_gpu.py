@@ -306,3 +306,16 @@ def test_offsets_past_32_bits(lib, Tq):
     call(lib, q, kk, vv, want, 400, 0, 3)
     check(q, kk, vv, want, 400, 0, 3)
     assert (o.float() - want.float()).abs().max() <= 4e-3
+
+
+def test_no_keys(lib):
+    """k_len 0 (k and v may be null): zeros in the rows that count, the others as they were."""
+    B, Tq, h, D = 3, 5, 4, 128
+    q = torch.randn(B, Tq, h, D, device="cuda").half()
+    o = torch.full_like(q, 7.0)
+    ql = torch.tensor([5, 0, 2], dtype=torch.int32, device="cuda")
+    kv = I3(1, 1, 1)                                       # an empty tensor's strides mean nothing
+    assert lib.da3b_attention_window(q.data_ptr(), s3(q), None, kv, None, kv, o.data_ptr(), s3(o), 0, B, Tq, 0, h, 2, D,
+                                     ql.data_ptr(), None, 3, 0, 1, 0.1, st()) == 0
+    for b, n in enumerate((5, 0, 2)):
+        assert (o[b, :n] == 0).all() and (o[b, n:] == 7.0).all()

@@ -159,6 +159,36 @@ def test_layernorm(lib, R, K, beta):
     check_quantised(q, bytes_of(s, R, K), y, 3e-6 * y.abs() + 3e-6 * 10, K)
 
 
+@pytest.mark.parametrize("R,K,pad,beta", [(5001, 1024, 0, True), (4000, 528, 8, False), (9001, 384, 16, True), (7003, 16, 0, True)])
+def test_layernorm_many_rows(lib, R, K, pad, beta):
+    """More rows than the device holds warps: each row as if it were normalised alone."""
+    g = gen(R + K)
+    x = torch.randn(R, K + pad, device="cuda", generator=g)[:, :K] * torch.rand(R, 1, device="cuda", generator=g) + 0.5
+    x = torch.nn.functional.pad(x, (0, pad), value=float("nan"))
+    gm = 1 + 0.2 * torch.randn(K, device="cuda", generator=g)
+    bt = 0.1 * torch.randn(K, device="cuda", generator=g)
+
+    def run(first, n):
+        q = torch.empty(n, K, dtype=torch.uint8, device="cuda")
+        s = torch.empty(lib.da3b_fp8_scale_bytes(n, K), dtype=torch.uint8, device="cuda")
+        assert lib.da3b_layernorm_fp8(x[first].data_ptr(), n, K, K + pad, gm.data_ptr(), bt.data_ptr() if beta else None,
+                                      1e-6, q.data_ptr(), K, s.data_ptr(), st()) == 0
+        return q, bytes_of(s, n, K)
+
+    q, b = run(0, R)
+    xd = x[:, :K].double()
+    d = xd - xd.mean(1, keepdim=True)
+    y = d / torch.sqrt((d * d).mean(1, keepdim=True) + 1e-6) * gm.double()
+    if beta:
+        y = y + bt.double()
+    # the mean is off by 2^-23 of the largest |x|, divided by the row's spread
+    err = 3e-6 * y.abs() + 3e-5 + 2.0 ** -22 * xd.abs().amax(1, keepdim=True) / d.pow(2).mean(1, keepdim=True).add(1e-6).sqrt() * gm.double().abs()
+    check_quantised(q, b, y, err, K)
+    for first, n in ((0, 128), (R // 2, 77), (R - 1, 1)):
+        q1, b1 = run(first, n)
+        assert torch.equal(q1, q[first:first + n]) and torch.equal(b1, b[first:first + n])
+
+
 def check_quantised(q, b, y, err, N):
     """Codes and scale bytes against y (64 bits) known to within err: the scale belongs to a
     block maximum inside the error, and each value is off by at most half a step."""

@@ -97,3 +97,20 @@ def test_attention_window_refusals(lib, change, rc):
     a = {**ATT, **change}
     args = [I3(*v) if isinstance(v, tuple) else v for v in a.values()]
     assert lib.da3b_attention_window(*args, None) == rc
+
+
+def test_buffers_without_rows_may_be_null(lib):
+    """As the tensors of an empty batch are: nothing is launched, and nothing is refused."""
+    a = {**QUANT, "rows": 0, "x": None, "q": None, "scales": None}
+    assert lib.da3b_quantize_fp8(*a.values(), None) == 0
+    a = {**LN, "rows": 0, "x": None, "q": None, "scales": None}
+    assert lib.da3b_layernorm_fp8(*a.values(), None) == 0
+    e = {**LIN, "M": 0, "x": None, "xs": None, "out": None}
+    assert lib.da3b_linear_fp8(*e.values(), None) == 0
+    assert lib.da3b_linear_fp8(*{**e, "w": None}.values(), None) == -100
+    a = {**{k: v for k, v in e.items() if k != "dt"}, "ldo": 32, "os": None}
+    assert lib.da3b_linear_fp8_q(*a.values(), None) == 0
+    assert lib.da3b_linear_fp8_resid_f32(None, 0, 100, 112, None, P, 30, 112, P, None, None, None, 30, None) == 0
+    for change in (dict(nseq=0), dict(q_len=0)):
+        a = {**ATT, **change, "q": None, "out": None}
+        assert lib.da3b_attention_window(*[I3(*v) if isinstance(v, tuple) else v for v in a.values()], None) == 0
