@@ -35,6 +35,12 @@ namespace {
 //              its dims contiguous: an MN-major operand), then S_t = Q_t K^T two tiles on;
 //   warps 4..  softmax, four a query tile: thread = row (its TMEM lane), the row's scores in
 //              registers, one pass; P back to tensor memory.
+// A CTA that is through its loads takes over the item of a CTA that has not been launched yet
+// (cluster launch control), so that barriers and tensor memory are set up once, and the next
+// item's queries, keys and scores are on their way while the softmax warps write this one's
+// rows. The order stays the grid's, and no counter in memory has to be reset. Two prompts of
+// 8192 tokens, 16 heads of 128, a window of 1024: 183 us with a CTA an item, 148 so (a window
+// of 64: 82 and 44; 64 views of 1370 tokens, 16 heads of 64: 835 and 710).
 // Tensor memory holds two S_t for each query tile, taken in turn, and P_t lies over its S_t:
 // the scores of the next key tile are there when a softmax is done, and one barrier each way
 // is enough. What bounds it is that softmax, a chain of its own: 16384 keys, 9 x 16 CTAs, take
@@ -42,7 +48,7 @@ namespace {
 // products, 660 (968) without the exponentials, and 540 (536) without both, which is what
 // the waits, the trip from and to tensor memory and the maximum take. Several query tiles
 // fill each other's waits; tensor memory has no room for more of them. Full attention of 4096
-// tokens runs at 694 and 1082 TFLOP/s. Taken otherwise: P_t over a single S_t (746 us against
+// tokens runs at 743 and 1130 TFLOP/s. Taken otherwise: P_t over a single S_t (746 us against
 // 793 in that measure with four query tiles, but 114 against 86 for a new view of 1297
 // tokens, whose items then fill 96 SMs), S_t and P_t in columns of their own (802 us, 90), two
 // softmax threads a row (1057 us), one issuing warp for all query tiles (its waits, about
@@ -66,7 +72,7 @@ struct WinCfg {
   static constexpr int kQTile = 128 * D * 2, kTile = kKT * D * 2;  // bytes of a Q and of a K or V tile
   static constexpr int kStage = 2 * kTile;          // a V tile and a K tile
   static constexpr int kRing = D == 64 ? 10 : 5, kRingBytes = kRing * kStage;
-  static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 512;
+  static constexpr int kSmem = 1024 + kNT * kQTile + kRingBytes + 640;
   static constexpr uint32_t kColO = 2 * kNT * kKT;  // behind two S_t each
   static_assert(kColO + kNT * D <= 512, "tensor memory");
   // a CTA's share of a split item: O rows, then (m, l), over the Q tiles and the ring
@@ -186,6 +192,24 @@ __device__ __forceinline__ void take_o(uint32_t taddr, bool any, uint32_t (&w)[3
   }
 }
 
+// Transposes 4 x 4 chunks over four neighbouring lanes: lane j's u[i] becomes lane i's u[j].
+__device__ __forceinline__ void turn4(uint4 (&u)[4], int lane) {
+  auto swap = [&](uint4& x, uint4& y, int by) {
+    const bool up = lane & by;
+    uint4 give = up ? x : y;
+    give.x = __shfl_xor_sync(0xffffffffu, give.x, by);
+    give.y = __shfl_xor_sync(0xffffffffu, give.y, by);
+    give.z = __shfl_xor_sync(0xffffffffu, give.z, by);
+    give.w = __shfl_xor_sync(0xffffffffu, give.w, by);
+    if (up) x = give;
+    else y = give;
+  };
+  swap(u[0], u[1], 1);
+  swap(u[2], u[3], 1);
+  swap(u[0], u[2], 2);
+  swap(u[1], u[3], 2);
+}
+
 // Shared-memory descriptor of an MN-major operand tile in 128B-swizzled rows of 64 values:
 // 1024 bytes between groups of eight k rows, lbo bytes between 64-wide column chunks.
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
@@ -205,6 +229,30 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Work that is left in the grid: asks for the launch of a CTA that has not begun to be
+// cancelled, so that this one takes its item (16 bytes at answer, one phase of bar). Not
+// asked again once an answer was no.
+__device__ __forceinline__ void take_launch(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// blockIdx.x of the cancelled CTA, -1 for none.
+__device__ __forceinline__ int launch_taken(const uint4* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}\n"
+      : "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
 }
 
 // What the rows of one query tile see: tokens [i0, i0 + n) of a sequence at positions from
@@ -262,6 +310,41 @@ struct Columns {
   __device__ bool mixed(int v0, int keys) const { return v0 < front && front < v0 + keys; }
 };
 
+// One unit of work: up to qt query tiles of a group of heads of a sequence, and of their key
+// tiles the share that one CTA of a cluster of nsplit takes. Items are numbered so that a
+// sequence's last tokens come first: where the left side is not limited they have the most
+// keys.
+template <int KT>
+struct alignas(16) Item {
+  int b, h0, hk, ql, kl, i0;
+  int nt;        // query tiles with rows (-1: not an item, there is no more work)
+  int lo, hi;    // columns that the windows reach
+  int n0, n_all; // first key tile and their number
+  Columns cols;
+  __device__ Item(const AttnWindow& a, int item, int split, int nsplit, int g, int tokens, int qt, int tiles)
+      : b(item / tiles / (a.heads / g)),
+        h0(item / tiles % (a.heads / g) * g),
+        hk(h0 / (a.heads / a.kv_heads)),
+        ql(a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len),
+        kl(a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len),
+        i0((tiles - 1 - item % tiles) * qt * tokens),
+        cols(a.sinks, Span(i0, tokens, ql, kl, a.left, a.right).lo_min) {
+    nt = i0 < ql ? min(qt, (ql - i0 + tokens - 1) / tokens) : 0;
+    const int hi_key = nt > 0 ? Span(i0 + (nt - 1) * tokens, tokens, ql, kl, a.left, a.right).hi_max : -1;
+    hi = hi_key + cols.shift();
+    lo = Span(i0, tokens, ql, kl, a.left, a.right).lo_min + cols.shift();
+    const int n_cols = hi_key < 0 ? 0 : hi / KT + 1;
+    n0 = static_cast<int>(static_cast<int64_t>(split) * n_cols / nsplit);
+    n_all = static_cast<int>(static_cast<int64_t>(split + 1) * n_cols / nsplit) - n0;
+  }
+  __device__ Span span(const AttnWindow& a, int tokens, int t) const {
+    Span sp(i0 + t * tokens, t < nt ? tokens : 0, ql, kl, a.left, a.right);
+    sp.shift(cols.shift());
+    return sp;
+  }
+  __device__ int col0(int n) const { return (n0 + n) * KT; }
+};
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -275,8 +358,14 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   uint8_t* sQ = smem;                       // [NT]
   // the ring: load i brings V of tile i - 2 and K of tile i, where there are such tiles
   uint8_t* sKV = sQ + NT * C::kQTile;       // [kRing] V, K
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(sKV + C::kRingBytes);
-  uint64_t* kv_full = q_full + 1;           // [kRing]
+  Item<KT>* items = reinterpret_cast<Item<KT>*>(sKV + C::kRingBytes);  // [2] the current one and the next
+  uint4* answer = reinterpret_cast<uint4*>(items + 2);  // to the request for another item
+  uint64_t* answered = reinterpret_cast<uint64_t*>(answer + 1);
+  uint64_t* item_full = answered + 1;       // [2]
+  uint64_t* item_free = item_full + 2;      // [2] done with by every warp that works
+  uint64_t* q_full = item_free + 2;
+  uint64_t* q_free = q_full + 1;            // the item's last scores are complete (every issuing warp)
+  uint64_t* kv_full = q_free + 1;           // [kRing]
   uint64_t* kv_empty = kv_full + C::kRing;  // [kRing] (every issuing warp)
   // one barrier for the even and one for the odd ones of the tiles that query tile t sees:
   uint64_t* s_full = kv_empty + C::kRing;   // [NT][2] S_t complete (and the product two before)
@@ -285,34 +374,18 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2 * NT);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a cluster of nsplit CTAs shares an item's key tiles; a sequence's last tokens come first:
-  // where the left side is not limited they have the most keys
-  const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
-  const int hgs = a.heads / g;
+  // a cluster of nsplit CTAs shares an item's key tiles
+  const int split = static_cast<int>(blockIdx.x) % nsplit, item0 = static_cast<int>(blockIdx.x) / nsplit;
   pdl_wait();
-  const int tile0 = tiles - 1 - item % tiles, hg = item / tiles % hgs, b = item / tiles / hgs;
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-  const int kl = a.k_lens ? min(max(a.k_lens[b], 0), a.k_len) : a.k_len;
-  const int i0 = tile0 * qt * tokens, h0 = hg * g, hk = h0 / (a.heads / a.kv_heads);
-  if (i0 >= ql) return;
-  const int nt = min(qt, (ql - i0 + tokens - 1) / tokens);  // query tiles with rows
-  const Span first(i0, tokens, ql, kl, a.left, a.right);
-  const Columns cols(a.sinks, first.lo_min);
-  auto span = [&](int t) {
-    Span sp(i0 + t * tokens, t < nt ? tokens : 0, ql, kl, a.left, a.right);
-    sp.shift(cols.shift());
-    return sp;
-  };
-  // columns that the windows reach, tiles of the item, and of this CTA
-  const int hi_key = Span(i0 + (nt - 1) * tokens, tokens, ql, kl, a.left, a.right).hi_max;
-  const int hi = hi_key + cols.shift(), lo = first.lo_min + cols.shift();
-  const int n_cols = hi_key < 0 ? 0 : hi / KT + 1;
-  const int n0 = static_cast<int>(static_cast<int64_t>(split) * n_cols / nsplit);
-  const int n_all = static_cast<int>(static_cast<int64_t>(split + 1) * n_cols / nsplit) - n0;
-  auto col0 = [&](int n) { return (n0 + n) * KT; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_free, NT);
+    mbar_init(answered, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_free[i], 5 * NT);
+    }
     for (int s = 0; s < C::kRing; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], NT);
@@ -336,39 +409,71 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsCtl));
     if (warp == 0) {
-      if (lane == 0 && n_all > 0) {
+      if (lane == 0) {
         const uint32_t q_bytes = static_cast<uint32_t>(g * tokens) * 128;  // of one 64-wide box
-        mbar_arrive_expect_tx(q_full, q_bytes * (D / 64) * nt);
-        for (int t = 0; t < nt; ++t)
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sQ + t * C::kQTile + c * 16384, &tmQ, q_full, c * 64, h0, i0 + t * tokens, b);
-        auto load_tile = [&](uint8_t* dst, const CUtensorMap& whole, const CUtensorMap& eight, uint64_t* bar, int v0) {
-          for (int c = 0; c < D / 64; ++c) {
-            if (!cols.mixed(v0, KT)) {
-              tma_load_4d(dst + c * KT * 128, &whole, bar, c * 64, hk, cols.key(v0), b);
-            } else {
-              for (int j = 0; j < KT; j += 8)
-                tma_load_4d(dst + (c * KT + j) * 128, &eight, bar, c * 64, hk, cols.key(v0 + j), b);
+        int st = 0;
+        uint32_t par = 1, loads = 0, nq = 0;
+        bool ok = true;
+        int item = item0;
+        for (uint32_t k = 0;; ++k) {
+          ok = mbar_wait(&item_free[k & 1], ((k >> 1) & 1) ^ 1u, status, kStatusTimeoutEmpty);
+          if (!ok) break;
+          if (item < 0) items[k & 1].nt = -1;
+          else items[k & 1] = Item<KT>(a, item, split, nsplit, g, tokens, qt, tiles);
+          mbar_arrive(&item_full[k & 1]);
+          if (item < 0) break;
+          const Item<KT> it = items[k & 1];
+          auto load_tile = [&](uint8_t* dst, const CUtensorMap& whole, const CUtensorMap& eight, uint64_t* bar, int v0) {
+            for (int c = 0; c < D / 64; ++c) {
+              if (!it.cols.mixed(v0, KT)) {
+                tma_load_4d(dst + c * KT * 128, &whole, bar, c * 64, it.hk, it.cols.key(v0), it.b);
+              } else {
+                for (int j = 0; j < KT; j += 8)
+                  tma_load_4d(dst + (c * KT + j) * 128, &eight, bar, c * 64, it.hk, it.cols.key(v0 + j), it.b);
+              }
+            }
+          };
+          if (it.n_all > 0) {
+            ok = mbar_wait(q_free, (nq & 1) ^ 1u, status, kStatusTimeoutEmpty);
+            if (ok) {
+              mbar_arrive_expect_tx(q_full, q_bytes * (D / 64) * it.nt);
+              for (int t = 0; t < it.nt; ++t)
+                for (int c = 0; c < D / 64; ++c)
+                  tma_load_4d(sQ + t * C::kQTile + c * 16384, &tmQ, q_full, c * 64, it.h0, it.i0 + t * tokens, it.b);
+              ++nq;
+            }
+            for (int i = 0; i < it.n_all + 2 && ok; ++i) {
+              ok = mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty);
+              if (!ok) break;
+              uint8_t* dst = sKV + st * C::kStage;
+              const bool k_tile = i < it.n_all, v_tile = i >= 2;
+              mbar_arrive_expect_tx(&kv_full[st], (k_tile ? C::kTile : 0) + (v_tile ? C::kTile : 0));
+              if (k_tile) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], it.col0(i));
+              if (v_tile) load_tile(dst, tmV, tmV8, &kv_full[st], it.col0(i - 2));
+              ++loads;
+              if (++st == C::kRing) { st = 0; par ^= 1u; }
             }
           }
-        };
-        int st = 0;
-        uint32_t par = 1;
-        for (int i = 0; i < n_all + 2; ++i) {
-          if (!mbar_wait(&kv_empty[st], par, status, kStatusTimeoutEmpty)) {
-            drain(kv_full, C::kRing, i, status);
+          if (!ok || nsplit > 1) break;
+          // Ask for another item, not before this one's last tile is under way: work that is
+          // asked for early is not there for a CTA that runs out of it.
+          mbar_arrive_expect_tx(answered, 16);
+          take_launch(answer, answered);
+          ok = mbar_wait(answered, k & 1, status, kStatusTimeoutFull);
+          if (!ok) {  // as drain: the answer is written to this CTA's memory
+            for (int i = 0; i < 8 && !mbar_wait(answered, k & 1, status, kStatusTimeoutFull); ++i) {}
             break;
           }
-          uint8_t* dst = sKV + st * C::kStage;
-          const bool k = i < n_all, v = i >= 2;
-          mbar_arrive_expect_tx(&kv_full[st], (k ? C::kTile : 0) + (v ? C::kTile : 0));
-          if (k) load_tile(dst + C::kTile, tmK, tmK8, &kv_full[st], col0(i));
-          if (v) load_tile(dst, tmV, tmV8, &kv_full[st], col0(i - 2));
-          if (++st == C::kRing) { st = 0; par ^= 1u; }
+          item = launch_taken(answer);
+          fence_proxy_async_smem();  // read before another answer is written there
+        }
+        if (!ok) {
+          drain(kv_full, C::kRing, loads, status);
+          if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, status, kStatusTimeoutFull);
         }
       }
       __syncwarp();
-    } else if (warp <= NT && n_all > 0) {
+    } else if (warp <= NT) {
       // The whole warp runs this loop and one elected lane issues: addresses and descriptors
       // then stay in uniform registers, where the instructions want them. (With one lane in
       // the loop every product's operands were moved there one by one, and that set the
@@ -381,8 +486,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       const uint64_t qd = umma_desc_sw128(smem_u32(sQ) + t * C::kQTile);
       const uint64_t vd0 = desc_mn_sw128(smem_u32(sKV), KT * 128), kd0 = umma_desc_sw128(smem_u32(sKV) + C::kTile);
       const uint32_t tS = tmem + 2 * t * KT, tO = tmem + C::kColO + t * D;
-      const Seen<KT> see(span(t), a.sinks);
-      int ns = 0, np = 0;  // S and P V products issued
+      uint32_t ns = 0, np = 0;  // S and P V products issued
       auto issue_s = [&](int st) {
         const uint64_t kd = kd0 + st * (C::kStage >> 4);
         const uint32_t d = tS + (ns & 1) * KT;
@@ -397,192 +501,225 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         __syncwarp();
         ++ns;
       };
-      bool ok = mbar_wait_warp(q_full, 0, status, kStatusTimeoutFull);
+      bool ok = true;
       int st = 0;
-      uint32_t par = 0;
-      for (int i = 0; i < n_all + 2 && ok; ++i) {
-        ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
-        if (ok && i >= 2 && see.some(n0 + i - 2)) {
-          ok = mbar_wait_warp(&p_ready[2 * t + (np & 1)], (np >> 1) & 1, status, kStatusTimeoutFull);
-          if (ok) {
-            tc_fence_after();
-            const uint64_t vd = vd0 + st * (C::kStage >> 4);
-            const uint32_t p = tS + (np & 1) * KT;
-            if (one) {
+      uint32_t par = 0, nq = 0;
+      for (uint32_t k = 0; ok; ++k) {
+        ok = mbar_wait_warp(&item_full[k & 1], (k >> 1) & 1, status, kStatusTimeoutFull);
+        const Item<KT> it = items[k & 1];
+        if (!ok || it.nt < 0) break;
+        const Seen<KT> see(it.span(a, tokens, t), a.sinks);
+        const uint32_t np0 = np;
+        if (it.n_all > 0) ok = mbar_wait_warp(q_full, nq++ & 1, status, kStatusTimeoutFull);
+        for (int i = 0; i < it.n_all + 2 && it.n_all > 0 && ok; ++i) {
+          ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
+          if (ok && i >= 2 && see.some(it.n0 + i - 2)) {
+            ok = mbar_wait_warp(&p_ready[2 * t + (np & 1)], (np >> 1) & 1, status, kStatusTimeoutFull);
+            if (ok) {
+              tc_fence_after();
+              const uint64_t vd = vd0 + st * (C::kStage >> 4);
+              const uint32_t p = tS + (np & 1) * KT;
+              if (one) {
 #pragma unroll
-              for (int kk = 0; kk < KT / 16; ++kk)
-                umma_f16_tmem_a(tO, p + 8 * kk, vd + 128 * kk, id_o, (np > 0 || kk > 0) ? 1u : 0u);
-              umma_commit(&pv_done[2 * t + (np & 1)]);
+                for (int kk = 0; kk < KT / 16; ++kk)
+                  umma_f16_tmem_a(tO, p + 8 * kk, vd + 128 * kk, id_o, (np != np0 || kk > 0) ? 1u : 0u);
+                umma_commit(&pv_done[2 * t + (np & 1)]);
+              }
+              __syncwarp();
+              ++np;
             }
-            __syncwarp();
-            ++np;
           }
+          // behind the product that read the P_t in its place
+          if (ok && i < it.n_all && see.some(it.n0 + i)) {
+            tc_fence_after();
+            issue_s(st);
+          }
+          if (ok && one) {
+            umma_commit(&kv_empty[st]);
+            if (i == it.n_all - 1) umma_commit(q_free);
+          }
+          __syncwarp();
+          if (++st == C::kRing) { st = 0; par ^= 1u; }
         }
-        // behind the product that read the P_t in its place
-        if (ok && i < n_all && see.some(n0 + i)) {
-          tc_fence_after();
-          issue_s(st);
-        }
-        if (ok && one) umma_commit(&kv_empty[st]);
+        if (nsplit > 1) break;
         __syncwarp();
-        if (++st == C::kRing) { st = 0; par ^= 1u; }
+        if (lane == 0) mbar_arrive(&item_free[k & 1]);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
     const int t = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
-    const Seen<KT> see(span(t), a.sinks);
-    // tiles with keys that no row of the CTA sees, and the tiles that need no look: seen whole
-    // by this query tile, and by its windows alone
-    const int fix0 = lo > a.sinks ? a.sinks / KT : 1, fix1 = lo > a.sinks ? (lo - 1) / KT : 0;
-    const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;
-    const int plain0 = max(see.whole0, fix1 + 1), plain1 = min(min(see.whole1, see.last), fix2 < 0 ? see.whole1 : fix2 - 1);
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tS0 = tmem + 2 * t * KT + lanes, tO = tmem + C::kColO + t * D + lanes;
     const float c = a.scale * 1.4426950408889634f;
-    const int p = kl - ql + i0 + t * tokens + r / g;   // this row's position
-    const int row_hi = min(kl - 1, p + a.right) + cols.shift(), row_lo = p - a.left + cols.shift();  // columns
-    float m = -INFINITY, l = 0.f;
-    int cnt = 0, st = 1;
-    uint32_t par = 0;
+    int cnt = 0, st = C::kRing - 1;
+    uint32_t par = 1;
     bool ok = true;
-    for (int n = 0; n < n_all && ok; ++n) {
-      if (++st == C::kRing) { st = 0; par ^= 1u; }  // the stage of this tile's V
-      const bool plain = n0 + n >= plain0 && n0 + n <= plain1;
-      if (!plain && !see.some(n0 + n)) continue;
-      const int v0 = col0(n);
-      const uint32_t tS = tS0 + (cnt & 1) * KT;  // S_t, then P_t
-      ok = mbar_wait_warp(&s_full[2 * t + (cnt & 1)], (cnt >> 1) & 1, status, kStatusTimeoutAccum);
-      if (!ok) break;
-      tc_fence_after();
-      float s[KT];
-      load_cols<KT>(tS, s);
-      // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
-      if (!plain && (n0 + n == fix2 || (n0 + n >= fix0 && n0 + n <= fix1))) {
-        ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
-        if (!ok) break;
-        const int v = v0 + r;
-        if (r < KT && (v > hi || (v < lo && v >= a.sinks))) {
-          uint4* row = reinterpret_cast<uint4*>(sKV + st * C::kStage + r * 128);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) row[(i >> 3) * (KT * 8) + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
+    auto advance = [&]() {
+      if (++st == C::kRing) { st = 0; par ^= 1u; }
+    };
+    for (uint32_t k = 0;; ++k) {
+      ok = mbar_wait_warp(&item_full[k & 1], (k >> 1) & 1, status, kStatusTimeoutFull);
+      if (nsplit == 1 && (!ok || items[k & 1].nt < 0)) break;
+      const int cnt0 = cnt;
+      float m = -INFINITY, l = 0.f;
+      if (ok) {
+        const Item<KT> it = items[k & 1];
+        const Seen<KT> see(it.span(a, tokens, t), a.sinks);
+        const int n0 = it.n0, n_all = it.n_all, lo = it.lo, hi = it.hi;
+        // tiles with keys that no row of the CTA sees, and the tiles that need no look: seen whole
+        // by this query tile, and by its windows alone
+        const int fix0 = lo > a.sinks ? a.sinks / KT : 1, fix1 = lo > a.sinks ? (lo - 1) / KT : 0;
+        const int fix2 = (hi + 1) % KT != 0 ? hi / KT : -1;
+        const int plain0 = max(see.whole0, fix1 + 1);
+        const int plain1 = min(min(see.whole1, see.last), fix2 < 0 ? see.whole1 : fix2 - 1);
+        const int p = it.kl - it.ql + it.i0 + t * tokens + r / g;   // this row's position, and its columns
+        const int row_hi = min(it.kl - 1, p + a.right) + it.cols.shift(), row_lo = p - a.left + it.cols.shift();
+        if (n_all > 0) {  // the loads bring V two behind K
+          advance();
+          advance();
         }
-        fence_proxy_async_smem();
-      }
-      tmem_wait_ld();
-      landed<KT>(s);
-      if (!plain && !see.whole(n0 + n)) {
-        // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
-        const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
+        for (int n = 0; n < n_all && ok; ++n) {
+          advance();  // the stage of this tile's V
+          const bool plain = n0 + n >= plain0 && n0 + n <= plain1;
+          if (!plain && !see.some(n0 + n)) continue;
+          const int v0 = (n0 + n) * KT;
+          const uint32_t tS = tS0 + (cnt & 1) * KT;  // S_t, then P_t
+          ok = mbar_wait_warp(&s_full[2 * t + (cnt & 1)], (cnt >> 1) & 1, status, kStatusTimeoutAccum);
+          if (!ok) break;
+          tc_fence_after();
+          float s[KT];
+          load_cols<KT>(tS, s);
+          // keys that no row of the CTA sees: their V rows count as zero, whatever they hold
+          if (!plain && (n0 + n == fix2 || (n0 + n >= fix0 && n0 + n <= fix1))) {
+            ok = mbar_wait_warp(&kv_full[st], par, status, kStatusTimeoutFull);
+            if (!ok) break;
+            const int v = v0 + r;
+            if (r < KT && (v > hi || (v < lo && v >= a.sinks))) {
+              uint4* row = reinterpret_cast<uint4*>(sKV + st * C::kStage + r * 128);
 #pragma unroll
-        for (int w = 0; w < (KT + 31) / 32; ++w) {
-          const uint32_t bits = below(x1 + 1 - 32 * w) & (~below(x0 - 32 * w) | below(x2 - 32 * w));
-#pragma unroll
-          for (int i = 0; i < 32 && 32 * w + i < KT; ++i) s[32 * w + i] = bits >> i & 1u ? s[32 * w + i] : -INFINITY;
-        }
-      }
-      float m8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[KT - 8 + i]);
-#pragma unroll
-      for (int i = 8; i < KT - 8; i += 16)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
-      const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
-      const bool raise = cnt == 0 || (mt - m) * c > kRaise;
-      const float alpha = raise ? ex2((m - mt) * c) : 1.f;
-      if (raise) m = mt;
-      const float mc = m == -INFINITY ? 0.f : m * c;
-      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      uint32_t pk[KT / 2];
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) {
-        const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(-mc, -mc));
-        const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
-        sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-        pk[i] = pack2<BF16>(e.x, e.y);
-      }
-      const float2 s2 = __fadd2_rn(sum[0], sum[1]);
-      // O_t is rescaled behind the last tile's product (the one before that is complete: S_t of
-      // this tile was issued after it, so no phase of the barrier is missed)
-      if (cnt > 0 && __any_sync(0xffffffffu, raise)) {
-        ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll 1
-        for (int i = 0; i < D; i += 16) {
-          uint32_t w[16];
-          tmem_ld16(tO + i, w);
+              for (int i = 0; i < D / 8; ++i) row[(i >> 3) * (KT * 8) + (i & 7)] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+          }
           tmem_wait_ld();
+          landed<KT>(s);
+          if (!plain && !see.whole(n0 + n)) {
+            // visible columns of this row: [x0, x1] and [0, x2) of the tile, up to x1
+            const int x1 = row_hi - v0, x0 = row_lo - v0, x2 = a.sinks - v0;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
-          tmem_st16(tO + i, w);
-        }
-        l *= alpha;
-      }
-      l += s2.x + s2.y;
-      store_words<KT / 2>(tS, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[2 * t + (cnt & 1)]);
-      ++cnt;
-    }
-    if (ok && cnt > 0) {
-      ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
-      tc_fence_after();
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    if (nsplit == 1) {
-      // O / l, 64 columns at a time through this warp's part of its (now idle) Q tile. A row
-      // that saw no key still has m = -inf and is zero (exp2_cubic gives its masked scores
-      // 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
-      const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
-      uint8_t* stg = sQ + t * C::kQTile + q * 4096;
-      const int rows = ok ? span(t).n * g : 0;
+            for (int w = 0; w < (KT + 31) / 32; ++w) {
+              const uint32_t bits = below(x1 + 1 - 32 * w) & (~below(x0 - 32 * w) | below(x2 - 32 * w));
+#pragma unroll
+              for (int i = 0; i < 32 && 32 * w + i < KT; ++i)
+                s[32 * w + i] = bits >> i & 1u ? s[32 * w + i] : -INFINITY;
+            }
+          }
+          float m8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) m8[i] = fmaxf(s[i], s[KT - 8 + i]);
+#pragma unroll
+          for (int i = 8; i < KT - 8; i += 16)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m8[j] = fmax3(m8[j], s[i + j], s[i + 8 + j]);
+          const float mt = fmaxf(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), m8[6]), m8[7]);
+          const bool raise = (mt - m) * c > kRaise;  // the first finite one, too; -inf - -inf: no
+          const float alpha = raise ? ex2((m - mt) * c) : 1.f;
+          if (raise) m = mt;
+          const float mc = m == -INFINITY ? 0.f : m * c;
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[KT / 2];
+#pragma unroll
+          for (int i = 0; i < KT / 2; ++i) {
+            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(c, c), make_float2(-mc, -mc));
+            const float2 e = (i & 3) == 0 ? exp2_cubic(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+            pk[i] = pack2<BF16>(e.x, e.y);
+          }
+          const float2 s2 = __fadd2_rn(sum[0], sum[1]);
+          // O_t is rescaled behind the last tile's product, where there is one (l is 0 before
+          // the first tile only). The product before that is complete: S_t of this tile was
+          // issued after it, so no phase of the barrier is missed.
+          if (__any_sync(0xffffffffu, raise && l != 0.f)) {
+            ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-      for (int ch = 0; ch < D / 64; ++ch) {
+            for (int i = 0; i < D; i += 16) {
+              uint32_t w[16];
+              tmem_ld16(tO + i, w);
+              tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+              tmem_st16(tO + i, w);
+            }
+            l *= alpha;
+          }
+          l += s2.x + s2.y;
+          store_words<KT / 2>(tS, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[2 * t + (cnt & 1)]);
+          ++cnt;
+        }
+      }
+      if (ok && cnt > cnt0) {
+        ok = mbar_wait_warp(&pv_done[2 * t + ((cnt - 1) & 1)], ((cnt - 1) >> 1) & 1, status, kStatusTimeoutAccum);
+        tc_fence_after();
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (nsplit == 1) {
+        // O / l. A row that saw no key still has m = -inf and is zero (exp2_cubic gives its
+        // masked scores 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
+        const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
+        const Item<KT> it = items[k & 1];
+        const bool mine = ok && r < it.span(a, tokens, t).n * g;
+        const int64_t off = it.b * a.os.seq + static_cast<int64_t>(it.i0 + t * tokens + r / g) * a.os.tok +
+                            static_cast<int64_t>(it.h0 + r % g) * a.os.head;
+#pragma unroll 1
+        for (int ch = 0; ch < D / 32; ++ch) {
           uint32_t w[32];
-          take_o(tO + 64 * ch + 32 * h, cnt > 0, w);
+          take_o(tO + 32 * ch, cnt > cnt0, w);
+          uint4 u[4];  // 16-byte chunks of this lane's row
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint4 u;
-            uint32_t* uw = reinterpret_cast<uint32_t*>(&u);
+            uint32_t* uw = reinterpret_cast<uint32_t*>(&u[i]);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               uw[j] = pack2<BF16>(__uint_as_float(w[8 * i + 2 * j]) * inv, __uint_as_float(w[8 * i + 2 * j + 1]) * inv);
-            *reinterpret_cast<uint4*>(stg + lane * 128 + (((4 * h + i) ^ (lane & 7)) << 4)) = u;
+          }
+          // four lanes exchange so that they hold a row's four chunks, one row after the other
+          turn4(u, lane);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int from = (lane & 28) + i;
+            const int64_t o = __shfl_sync(0xffffffffu, off, from);
+            if (__shfl_sync(0xffffffffu, mine, from))
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + o + 32 * ch + 8 * (lane & 3)) = u[i];
           }
         }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int row = 4 * k + (lane >> 3), ci = lane & 7, rr = q * 32 + row;
-          const uint4 u = *reinterpret_cast<const uint4*>(stg + row * 128 + ((ci ^ (row & 7)) << 4));
-          const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + rr / g) * a.os.tok +
-                              static_cast<int64_t>(h0 + rr % g) * a.os.head + ch * 64 + ci * 8;
-          if (rr < rows) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + off) = u;
-        }
-        __syncwarp();
-      }
-    } else {
-      // this CTA's share of the row, over the Q tiles and the ring (idle once every tile's
-      // products are complete: all softmax warps come here): O, 16-byte chunks XOR-swizzled
-      // by row, then (m, l)
-      asm volatile("bar.sync 1, %0;" ::"n"(128 * NT) : "memory");
-      float4* part = reinterpret_cast<float4*>(smem) + (t * 128 + r) * (D / 4);
+        tc_fence_before();  // O_t has been read before the next item's first P_t is ready
+      } else {
+        // this CTA's share of the row, over the Q tiles and the ring (idle once every tile's
+        // products are complete: all softmax warps come here): O, 16-byte chunks XOR-swizzled
+        // by row, then (m, l)
+        asm volatile("bar.sync 1, %0;" ::"n"(128 * NT) : "memory");
+        float4* part = reinterpret_cast<float4*>(smem) + (t * 128 + r) * (D / 4);
 #pragma unroll 1
-      for (int ch = 0; ch < D / 32; ++ch) {
-        uint32_t w[32];
-        take_o(tO + 32 * ch, cnt > 0, w);
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t w[32];
+          take_o(tO + 32 * ch, cnt > cnt0, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          part[(8 * ch + i) ^ (r & 7)] = make_float4(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]),
-                                                     __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3]));
+          for (int i = 0; i < 8; ++i)
+            part[(8 * ch + i) ^ (r & 7)] = make_float4(__uint_as_float(w[4 * i]), __uint_as_float(w[4 * i + 1]),
+                                                       __uint_as_float(w[4 * i + 2]), __uint_as_float(w[4 * i + 3]));
+        }
+        reinterpret_cast<float2*>(smem + C::kShareO)[t * 128 + r] = make_float2(m, l);
       }
-      reinterpret_cast<float2*>(smem + C::kShareO)[t * 128 + r] = make_float2(m, l);
+      if (!ok || nsplit > 1) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_free[k & 1]);
     }
   }
   if (nsplit > 1) {
@@ -591,10 +728,11 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
     // takes four rows at a time, eight lanes each.
     cluster_sync();
     if (warp >= 4) {
+      const Item<KT> it = items[0];
       const float c = a.scale * 1.4426950408889634f;
       const uint32_t part = smem_u32(smem), ml = part + C::kShareO;
       const int sub = lane & 7;
-      const int last = ((nt - 1) * 128) + min(tokens, ql - i0 - (nt - 1) * tokens) * g;
+      const int last = ((it.nt - 1) * 128) + min(tokens, it.ql - it.i0 - (it.nt - 1) * tokens) * g;
       for (int row = (split * 4 * NT + warp - 4) * 4 + (lane >> 3); row < last; row += nsplit * 16 * NT) {
         const int t = row >> 7, r = row & 127;
         if (r >= tokens * g) continue;
@@ -626,8 +764,8 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
           }
         }
         const float inv = mx == -INFINITY && sum == sum ? 0.f : 1.f / sum;
-        const int64_t off = b * a.os.seq + static_cast<int64_t>(i0 + t * tokens + r / g) * a.os.tok +
-                            static_cast<int64_t>(h0 + r % g) * a.os.head + 4 * sub;
+        const int64_t off = it.b * a.os.seq + static_cast<int64_t>(it.i0 + t * tokens + r / g) * a.os.tok +
+                            static_cast<int64_t>(it.h0 + r % g) * a.os.head + 4 * sub;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + off + 32 * j) =
@@ -706,13 +844,14 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
       return -5;
     attr_set.fetch_or(uint64_t(1) << (dev & 63));
   }
-  // Query tiles a CTA, and a split of its key tiles over a cluster: whatever makes the call
-  // shortest. CTAs run one an SM, so a call takes its waves of CTAs times a CTA's time, with
-  // the times measured (ns a key tile for 1, 2, .. query tiles; setup and joining about 4 and
-  // 5 us). A view of 1297 tokens and 16 heads over 7800 keys: 64 items of three query tiles,
-  // each split in two, take 85 us; unsplit 149, 96 unsplit items of two query tiles 133.
+  // Query tiles an item, and a split of its key tiles over a cluster: whatever makes the call
+  // shortest. CTAs run one an SM, so a call takes its rounds of items times an item's time,
+  // with the times measured (ns a key tile for 1, 2, .. query tiles; about 4 us to set a CTA
+  // up, 1.3 for another item, 5 to join shares). A view of 1297 tokens and 16 heads over 7800
+  // keys: 64 items of three query tiles, each split in two, take 80 us; unsplit 149, 96 unsplit
+  // items of two query tiles 133.
   constexpr int64_t kTileNs[2][3] = {{560, 770, 865}, {720, 1000, 0}};
-  constexpr int64_t kSetupNs = 4000, kJoinNs = 5000;
+  constexpr int64_t kSetupNs = 4000, kNextNs = 1300, kJoinNs = 5000;
   int nsplit = 1, qt = C::kNT;
   int64_t best = 0;
   for (int n = C::kNT; n >= 1; --n) {
@@ -722,8 +861,9 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
     for (int ns = 1; ns <= 8 && (ns == 1 || keys >= 4 * ns); ++ns) {
       const int64_t at_once = clusters_at_once<D, BF16>(ns, dev);
       if (at_once <= 0) continue;
-      const int64_t cost = (items + at_once - 1) / at_once *
-                           ((keys + ns - 1) / ns * kTileNs[D == 128][n - 1] + kSetupNs + (ns > 1 ? kJoinNs : 0));
+      const int64_t rounds = (items + at_once - 1) / at_once, tile = kTileNs[D == 128][n - 1];
+      const int64_t cost = ns == 1 ? kSetupNs + rounds * (keys * tile + kNextNs)
+                                   : rounds * ((keys + ns - 1) / ns * tile + kSetupNs + kJoinNs);
       if (best == 0 || cost < best) {
         best = cost;
         nsplit = ns;

@@ -319,3 +319,31 @@ def test_no_keys(lib):
                                      ql.data_ptr(), None, 3, 0, 1, 0.1, st()) == 0
     for b, n in enumerate((5, 0, 2)):
         assert (o[b, :n] == 0).all() and (o[b, n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Tq,Tk,h,kvh,left,right,sinks", [
+    (50, 300, 420, 8, 4, 100, 0, 3),          # several items for each multiprocessor, of unlike lengths
+    (40, 131, 131, 12, 12, -1, -1, 0),
+    (30, 900, 900, 4, 1, 17, 5, 40),
+    (300, 33, 70, 2, 1, -1, 0, 0),
+])
+def test_more_items_than_multiprocessors(lib, B, Tq, Tk, h, kvh, left, right, sinks, D, dtype):
+    """Sequences of all lengths, 0 and 1 among them, with more queries than keys or fewer, and
+    NaN in every key past a length: what one item leaves behind must not reach the next."""
+    q, k, v = make(B, Tq, Tk, h, kvh, D, dtype, B + D)
+    g = torch.Generator().manual_seed(B)
+    kl = torch.randint(0, Tk + 1, (B,), generator=g, dtype=torch.int32)
+    ql = torch.minimum(torch.randint(0, Tq + 1, (B,), generator=g, dtype=torch.int32), kl + 3)
+    kl[:4], ql[:4] = torch.tensor([0, 1, Tk, Tk]), torch.tensor([2, 1, Tq, 0])
+    for b in range(B):
+        k[b, kl[b]:], v[b, kl[b]:] = float("nan"), float("inf")
+    kl, ql = kl.cuda(), ql.cuda()
+    o = torch.full_like(q, 7.0)
+    call(lib, q, k, v, o, left, right, sinks, ql, kl)
+    check(q, k, v, o, left, right, sinks, ql, kl, fill=7.0)
+    again = torch.full_like(q, 7.0)
+    call(lib, q, k, v, again, left, right, sinks, ql, kl)
+    assert torch.equal(o, again)              # whichever multiprocessor takes an item
+    assert lib.da3b_device_status() == 0
