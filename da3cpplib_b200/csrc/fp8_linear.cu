@@ -20,15 +20,16 @@
 //              buffer, stored (or, onto the residual, added) by TMA: the load-store unit,
 //              73 % busy with the pieces' reads and stores when the warps made them, only
 //              writes the buffer. Four warps an SM sub-partition hide each other's
-//              latencies: M = 87680, K = 1024, N = 4096 with GELU to f16 takes 400-430 us,
+//              latencies: M = 87680, K = 1024, N = 4096 with GELU to f16 takes 410-460 us,
 //              eight warps of 128 columns took 528-580.
 //
-// Bound: the MMAs (K = 1024: 4096 cycles a 256 x 256 tile at the full rate) and, one
-// accumulator to a CTA pair, the handover between them and the epilogue's reads. That shape
-// takes 343 us without an activation (2.14 PFLOP/s; the chip's power, at 1.5-1.6 GHz);
-// M = 21920 takes 87, K = 4096, N = 1024 79 (2.33 PFLOP/s). With GELU the epilogue's own
-// instructions (17 a value, two of them MUFU) are as long as the MMAs: 103 us at M = 21920,
-// 114 quantised. A ring of five stages: four and six measured the same.
+// Bound: long reductions by the chip's power (8192 x 8192 x 8192: 440 us or 2.5 PFLOP/s, the
+// MMAs at 92 % of their cycles but at 1.1 GHz), short ones by the MMAs (K = 1024: 4096 cycles a
+// 256 x 256 tile) and the handover of a pair's one accumulator to the epilogue and back, about
+// 1600 cycles: M = 87680, N = 4096 takes 315 us (2.3 PFLOP/s), M = 21920 85; K = 4096, N = 1024
+// 74. With GELU the epilogue's own instructions (17 a value, two of them MUFU) are as long as
+// the MMAs: 100 us at M = 21920, 96 quantised. A ring of five stages: four and six measured
+// the same.
 // Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
 #include <algorithm>
 #include <atomic>
@@ -372,22 +373,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsCtl));
+  // Producer and issuer loops run in the whole warp and one elected lane issues: addresses and
+  // descriptors then stay in uniform registers, where the instructions want them. With one
+  // lane in the loops every operand was moved there one by one, and that set the pace (M =
+  // 87680, K = 1024, N = 4096: 343 us against 315, 8192 x 8192 x 8192: 484 against 440).
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, loads = 0;
-      bool ok = true;
-      for (int t = unit; t < num_tiles && ok; t += units) {
-        const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, status, kStatusTimeoutEmpty)) { ok = false; break; }
-          ++loads;
-          const bool sf = (kb & 3) == 0;
+    const bool one = elect_one();
+    int stage = 0;
+    uint32_t phase = 0, loads = 0;
+    bool ok = true;
+    for (int t = unit; t < num_tiles && ok; t += units) {
+      const int mt = t / n_tiles * CG + static_cast<int>(rank), nt = t % n_tiles;
+      const int n0 = nt * C::kBN + static_cast<int>(rank) * 128;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        ok = mbar_wait_warp(&empty[stage], phase ^ 1u, status, kStatusTimeoutEmpty);
+        if (!ok) break;
+        ++loads;
+        const bool sf = (kb & 3) == 0;
+        uint8_t* da = sA + stage * C::kABytes;
+        uint8_t* db = sB + stage * C::kBBytes;
+        uint8_t* ds = sSf + stage * C::kSfBytes;
+        if (one) {
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], CG * (C::kStageBytes + (sf ? C::kSfBytes : 0)));
-          uint8_t* da = sA + stage * C::kABytes;
-          uint8_t* db = sB + stage * C::kBBytes;
-          uint8_t* ds = sSf + stage * C::kSfBytes;
-          const int n0 = nt * C::kBN + static_cast<int>(rank) * 128;
           if (CG == 2) {
             const uint32_t fb = mapa_shared(smem_u32(&full[stage]), 0);
             tma2_load_2d(da, &tmA, fb, kb * 128, mt * 128);
@@ -404,46 +411,56 @@ __global__ void __launch_bounds__(kThreads, 1)
               tma_load_2d(ds + 512, &tmSB, &full[stage], 0, (kb >> 2) * row_tiles_n + nt);
             }
           }
-          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
+        __syncwarp();
+        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
-      if (!ok && rank == 0) drain(full, C::kStages, loads, status);
     }
+    if (!ok && rank == 0 && lane == 0) drain(full, C::kStages, loads, status);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool one = elect_one();
+      const uint64_t ad0 = umma_desc_sw128(smem_u32(sA)), bd0 = umma_desc_sw128(smem_u32(sB));
       int stage = 0, it = 0;
       uint32_t phase = 0, group = 0;
       bool ok = true;
       for (int t = unit; t < num_tiles && ok; t += units, ++it) {
         const int acc = it % C::kAcc;
-        if (!mbar_wait(&tempty[acc], ((it / C::kAcc) & 1) ^ 1u, status, kStatusTimeoutAccumFree)) break;
+        ok = mbar_wait_warp(&tempty[acc], ((it / C::kAcc) & 1) ^ 1u, status, kStatusTimeoutAccumFree);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + acc * C::kBN;
         uint32_t sf = 0;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, status, kStatusTimeoutFull)) { ok = false; break; }
+          ok = mbar_wait_warp(&full[stage], phase, status, kStatusTimeoutFull);
+          if (!ok) break;
           tc_fence_after();
           if ((kb & 3) == 0) {
             sf = tmem + C::kColSf + (group++ % kSfBuffers) * C::kSfCols;
             const uint32_t ds = smem_u32(sSf + stage * C::kSfBytes);
+            if (one) {
 #pragma unroll
-            for (int i = 0; i < C::kSfATiles + C::kSfBTiles; ++i) copy_sf<CG>(sf + 4 * i, ds + 512 * i);
+              for (int i = 0; i < C::kSfATiles + C::kSfBTiles; ++i) copy_sf<CG>(sf + 4 * i, ds + 512 * i);
+            }
           }
-          const uint64_t ad = umma_desc_sw128(smem_u32(sA + stage * C::kABytes));
-          const uint64_t bd = umma_desc_sw128(smem_u32(sB + stage * C::kBBytes));
-          const uint32_t id = idesc_mxf8(128 * CG, C::kBN, kb & 3);
+          const uint64_t ad = ad0 + stage * (C::kABytes >> 4), bd = bd0 + stage * (C::kBBytes >> 4);
+          const uint32_t id = idesc_mxf8(128 * CG, C::kBN, 0) | (static_cast<uint32_t>(kb & 3) * ((1u << 4) | (1u << 29)));
+          if (one) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_mxf8<CG>(d, ad + 2 * k, bd + 2 * k, id, sf, sf + 4, (kb > 0 || k > 0) ? 1u : 0u);
-          if (CG == 2) umma2_commit_mc(&empty[stage], 0x3);
-          else umma_commit(&empty[stage]);
+            for (int k = 0; k < 4; ++k)
+              umma_mxf8<CG>(d, ad + 2 * k, bd + 2 * k, id, sf, sf + 4, (kb > 0 || k > 0) ? 1u : 0u);
+            if (CG == 2) umma2_commit_mc(&empty[stage], 0x3);
+            else umma_commit(&empty[stage]);
+          }
+          __syncwarp();
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
         }
-        if (ok) {
+        if (ok && one) {
           if (CG == 2) umma2_commit_mc(&tfull[acc], 0x3);
           else umma_commit(&tfull[acc]);
         }
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -577,19 +594,18 @@ int check_linear_fp8(const Fp8Linear& a) {
 }
 
 int linear_fp8(const Fp8Linear& a, int* status, cudaStream_t s) {
-  // The tile shape with the shorter time: waves of tiles times a tile's time. A k-block brings
-  // 32 KB into an SM with either, which takes 800 to 900 cycles (measured at K = 4096 on one
-  // and on all SMs; the tensor work takes 256 or 512), and a pair's one accumulator waits
-  // another 1600 cycles a tile for the epilogue to read it. Measured at N = 4096, K = 1024
-  // and M = 1370, 2740, 5480: single CTAs 15, 25, 43 us, pairs 13, 23, 33; at N = 1024,
-  // K = 4096, M = 1370: 17 and 21.
+  // The tile shape with the shorter time (ns): waves of tiles times a tile's k-blocks of 128,
+  // and the handover from one tile to the next, longer with a pair's one accumulator; pairs
+  // also take longer to set up. Measured at N = 4096, K = 1024 and M = 512, 1370, 2740, 5480,
+  // 21920: single CTAs 6.5, 11.3, 16.2, 28, 105 us, pairs 8.9, 12.3, 15.8, 23, 85; at N = 1024,
+  // K = 4096 and M = 1370, 2740: 13.6 and 22.8, 17.7 and 18.4.
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t sms = sm_count(dev), kb = (a.K + 127) / 128;
   const int64_t tiles1 = (static_cast<int64_t>(a.M) + 127) / 128 * ((a.N + 127) / 128);
   const int64_t tiles2 = (static_cast<int64_t>(a.M) + 255) / 256 * ((a.N + 255) / 256);
-  const int64_t time1 = (tiles1 + sms - 1) / sms * (kb * 800 + 300);
-  const int64_t time2 = (tiles2 + sms / 2 - 1) / (sms / 2) * (kb * 900 + 1600);
+  const int64_t time1 = 3800 + (tiles1 + sms - 1) / sms * (kb * 270 + 250);
+  const int64_t time2 = 4500 + (tiles2 + sms / 2 - 1) / (sms / 2) * (kb * 330 + 1300);
   return time2 <= time1 ? launch<2>(a, status, s) : launch<1>(a, status, s);
 }
 
