@@ -183,6 +183,7 @@ x, b = torch.randn(64, 128, device="cuda").half(), torch.randn(128, device="cuda
 q, s, qw, sw = e(64, 128), e(512), e(128, 128), e(512)
 w = torch.randn(128, 128, device="cuda")
 y, o, o1 = e(64, 128, t=torch.float16), e(64, 128, t=torch.float16), e(128, t=torch.float16)
+kv, o2 = torch.randn(3000, 128, device="cuda").half(), e(64, 128, t=torch.float16)
 
 def run():
     st = torch.cuda.current_stream().cuda_stream
@@ -192,7 +193,10 @@ def run():
     return [lib.da3b_quantize_fp8(w.data_ptr(), 2, 128, 128, 128, qw.data_ptr(), 128, sw.data_ptr(), st),
             lib.da3b_quantize_fp8(x.data_ptr(), 0, 64, 128, 128, q.data_ptr(), 128, s.data_ptr(), st),
             lib.da3b_linear_fp8(q.data_ptr(), 64, 128, 128, s.data_ptr(), qw.data_ptr(), 128, 128, sw.data_ptr(),
-                                b.data_ptr(), 0, y.data_ptr(), 0, 128, st), a(64, o), a(1, o1)]
+                                b.data_ptr(), 0, y.data_ptr(), 0, 128, st), a(64, o), a(1, o1),
+            lib.da3b_attention_window(y.data_ptr(), I3(8192, 128, 64), kv.data_ptr(), I3(1, 128, 64), kv.data_ptr(),
+                I3(1, 128, 64), o2.data_ptr(), I3(8192, 128, 64), 0, 1, 64, 3000, 2, 2, 64, None, None, -1, -1, 0,
+                0.125, st)]   # keys split over a cluster
 
 torch.cuda.synchronize()
 g = torch.cuda.CUDAGraph()
@@ -201,10 +205,10 @@ with torch.cuda.graph(g):
 print(rc)
 g.replay()
 torch.cuda.synchronize()
-got = [t.clone() for t in (y, o, o1)]
+got = [t.clone() for t in (y, o, o1, o2)]
 print(run())
 torch.cuda.synchronize()
-assert got[0].abs().max() > 0 and all(torch.equal(i, j) for i, j in zip(got, (y, o, o1)))
+assert all(t.abs().max() > 0 for t in got) and all(torch.equal(i, j) for i, j in zip(got, (y, o, o1, o2)))
 assert lib.da3b_device_status() == 0
 print("same")
 """
