@@ -256,7 +256,8 @@ DA3B_API int da3b_linear_fp8_resid_f32(const void* x, int M, int K, int ldx, con
  * packed q | k | v buffer or either order of tokens and heads is read in place. dtype 0
  * f16, 1 bf16; head_dim 64 or 128; heads a multiple of kv_heads: query head h reads key
  * head h / (heads / kv_heads). scale: finite, not negative.
- * Returns as the e4m3 linears do; nothing is allocated but the status word. */
+ * out may not overlap the inputs. Returns as the e4m3 linears do; nothing is allocated but
+ * the status word, and a stream may capture any call. */
 DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                    const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
                                    int dtype, int nseq, int q_len, int k_len, int heads, int kv_heads, int head_dim,
