@@ -1304,7 +1304,7 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
     if (reinterpret_cast<uintptr_t>(p) & 15) return -1;
   // 32-bit work counts inside
   if (static_cast<double>(nseq) * heads * q_len > 2147483647.0 * 8) return -1;
-  if (!writable_here(out)) return -104;
+  if (!usable_here({q, k_len > 0 ? k : nullptr, k_len > 0 ? v : nullptr, out, q_lens, k_lens})) return -104;
   int* st = device_status_word();
   if (!st) return -101;
   return attention_window(a, st, static_cast<cudaStream_t>(stream));

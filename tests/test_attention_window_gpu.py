@@ -177,6 +177,20 @@ def test_host_output_is_refused(lib):
     assert (o == 0).all()
 
 
+def test_host_inputs_are_refused(lib):
+    """Lengths in host memory, the likeliest of these mistakes, among them."""
+    q, k, v = make(1, 5, 9, 2, 2, 64, torch.float16, 6)
+    o = torch.full_like(q, 7.0)
+    host = torch.zeros(1 << 14, dtype=torch.uint8)
+    h = (host.data_ptr() + 63) // 64 * 64
+    n = torch.tensor([5], dtype=torch.int32)
+    a = [q.data_ptr(), s3(q), k.data_ptr(), s3(k), v.data_ptr(), s3(v), o.data_ptr(), s3(q), 0, 1, 5, 9, 2, 2, 64, None, None,
+         3, 0, 1, 0.125, st()]
+    for i, p in ((0, h), (2, h), (4, h), (15, n.data_ptr()), (16, n.data_ptr())):
+        assert lib.da3b_attention_window(*a[:i], p, *a[i + 1:]) == -104
+    assert lib.da3b_attention_window(*a) == 0 and (o != 7.0).any()
+
+
 def test_no_keys_at_all(lib):
     q, k, v = make(2, 33, 1, 2, 2, 64, torch.float16, 6)
     o = torch.full_like(q, 7.0)

@@ -326,6 +326,27 @@ def test_host_outputs_are_refused(lib):
     assert (host == 0).all()
 
 
+def test_host_inputs_are_refused(lib):
+    """So is an input there, the optional ones among them."""
+    M, K, N = 4, 128, 32
+    (xq, xs, xv, wq, ws, wv), bias = make_linear(lib, M, K, N, 1)
+    x, y = torch.randn(M, K, device="cuda"), torch.full((M, N), 7.0, device="cuda")
+    host = torch.zeros(1 << 16, dtype=torch.uint8)
+    h = (host.data_ptr() + 63) // 64 * 64
+    q, s = xq.data_ptr(), xs.data_ptr()
+    assert lib.da3b_quantize_fp8(h, 2, M, K, K, q, K, s, st()) == -104
+    ln = [x.data_ptr(), M, K, K, bias.data_ptr(), bias.data_ptr(), 1e-6, q, K, s, st()]
+    for i in (0, 4, 5):
+        assert lib.da3b_layernorm_fp8(*ln[:i], h, *ln[i + 1:]) == -104
+    lin = [q, M, K, xq.stride(0), s, wq.data_ptr(), N, wq.stride(0), ws.data_ptr(), bias.data_ptr()]
+    for i in (0, 4, 5, 8, 9):
+        a = lin[:i] + [h] + lin[i + 1:]
+        assert lib.da3b_linear_fp8(*a, 0, y.data_ptr(), 2, N, st()) == -104
+        assert lib.da3b_linear_fp8_resid_f32(*a, None, y.data_ptr(), N, st()) == -104
+    assert lib.da3b_linear_fp8_resid_f32(*lin, h, y.data_ptr(), N, st()) == -104
+    assert (y == 7.0).all()
+
+
 def test_linear_into_pinned_memory(lib):
     M, K, N = 40, 256, 96
     (xq, xs, xv, wq, ws, wv), bias = make_linear(lib, M, K, N, 1)
