@@ -46,7 +46,8 @@ namespace {
 // is enough. What bounds it is that softmax, a chain of its own: 16384 keys, 9 x 16 CTAs, take
 // 942 ns a step of 48 keys at head_dim 64 (1064 ns a step of 64 at 128), 858 (904) without the
 // products, 660 (968) without the exponentials, and 540 (536) without both, which is what
-// the waits, the trip from and to tensor memory and the maximum take. Several query tiles
+// the waits, the trip from and to tensor memory and the maximum take (since the first tile's
+// maximum lost its branch, 833 ns at head_dim 64). Several query tiles
 // fill each other's waits; tensor memory has no room for more of them. Full attention of 4096
 // tokens runs at 743 and 1130 TFLOP/s. Taken otherwise: P_t over a single S_t (746 us against
 // 793 in that measure with four query tiles, but 114 against 86 for a new view of 1297
@@ -827,7 +828,8 @@ int launch_tiles(const AttnWindow& a, int* status, cudaStream_t s) {
   const int tokens = 128 / g;
   CUtensorMap tq, tk, tv, tk8, tv8;
   if (map_4d(&tk8, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) ||
-      map_4d(&tv8, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) || map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
+      map_4d(&tv8, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, 8) ||
+      map_4d(&tq, a.q, a.qs, a.bf16, D, a.heads, a.q_len, a.nseq, g, tokens) ||
       map_4d(&tk, a.k, a.ks, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, C::kKT) ||
       map_4d(&tv, a.v, a.vs, a.bf16, D, a.kv_heads, a.k_len, a.nseq, 1, C::kKT))
     return -2;

@@ -585,7 +585,8 @@ int launch(const Fp8Linear& a, int* status, cudaStream_t s) {
 }  // namespace
 
 int check_linear_fp8(const Fp8Linear& a) {
-  if (a.K <= 0 || a.N <= 0 || a.M > kMostCount || a.N > kMostCount || a.K > kMostCount || a.ldx < a.K || a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.ldo < a.N ||
+  if (a.K <= 0 || a.N <= 0 || a.M > kMostCount || a.N > kMostCount || a.K > kMostCount || a.ldx < a.K ||
+      a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.ldo < a.N ||
       !aligned(a.x, 16) || !aligned(a.w, 16) || !aligned(a.xs, 16) || !aligned(a.ws, 16) ||
       !aligned(a.out, out_size(a.kind)) || !aligned(a.bias, 4) || !aligned(a.scale, 4))
     return -1;
