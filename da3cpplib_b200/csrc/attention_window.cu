@@ -546,6 +546,8 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_free[k & 1]);
       }
+      // every load of the item has landed; the softmax warps write their shares over them
+      if (nsplit > 1) asm volatile("bar.sync 1, %0;" ::"n"(160 * NT) : "memory");
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoft));
@@ -702,10 +704,12 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         }
         tc_fence_before();  // O_t has been read before the next item's first P_t is ready
       } else {
-        // this CTA's share of the row, over the Q tiles and the ring (idle once every tile's
-        // products are complete: all softmax warps come here): O, 16-byte chunks XOR-swizzled
-        // by row, then (m, l)
-        asm volatile("bar.sync 1, %0;" ::"n"(128 * NT) : "memory");
+        // this CTA's share of the row, over the Q tiles and the ring: O, 16-byte chunks
+        // XOR-swizzled by row, then (m, l). They are idle once every product is complete, which
+        // the softmax warps know, and every load, which the issuing warps know: a tile between
+        // the sinks and the windows is loaded although no row sees it, and no product waits
+        // for one at the end of the share.
+        asm volatile("bar.sync 1, %0;" ::"n"(160 * NT) : "memory");
         float4* part = reinterpret_cast<float4*>(smem) + (t * 128 + r) * (D / 4);
 #pragma unroll 1
         for (int ch = 0; ch < D / 32; ++ch) {
