@@ -373,6 +373,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   uint64_t* p_ready = s_full + 2 * NT;      // [NT][2] P_t written, O_t rescaled, V rows zeroed (4 warps)
   uint64_t* pv_done = p_ready + 2 * NT;     // [NT][2] P_t V complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2 * NT);
+  uint32_t* gave_up = tmem_slot + 1;        // not 0: a wait of this CTA ran out
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a cluster of nsplit CTAs shares an item's key tiles
@@ -380,6 +381,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
   pdl_wait();
 
   if (threadIdx.x == 0) {
+    *gave_up = 0;
     mbar_init(q_full, 1);
     mbar_init(q_free, NT);
     mbar_init(answered, 1);
@@ -471,6 +473,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         if (!ok) {
           drain(kv_full, C::kRing, loads, status);
           if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, status, kStatusTimeoutFull);
+          *gave_up = 1;
         }
       }
       __syncwarp();
@@ -546,6 +549,7 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_free[k & 1]);
       }
+      if (!ok) *gave_up = 1;
       // every load of the item has landed; the softmax warps write their shares over them
       if (nsplit > 1) asm volatile("bar.sync 1, %0;" ::"n"(160 * NT) : "memory");
     }
@@ -726,13 +730,17 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_free[k & 1]);
     }
+    if (!ok) *gave_up = 1;
   }
   if (nsplit > 1) {
     // Join the shares in rank order (the result does not depend on who finished first):
     // with M the largest m, O = sum 2^((m_s - M) c) O_s / sum 2^((m_s - M) c) l_s. A warp
-    // takes four rows at a time, eight lanes each.
+    // takes four rows at a time, eight lanes each. Nothing is joined once a wait of any CTA of
+    // the cluster ran out: its share is not one, and its item may never have been written.
     cluster_sync();
-    if (warp >= 4) {
+    uint32_t any_gave_up = 0;
+    for (int i = 0; i < nsplit; ++i) any_gave_up |= __float_as_uint(ld_dsmem_f1(mapa_shared(smem_u32(gave_up), i)));
+    if (warp >= 4 && any_gave_up == 0) {
       const Item<KT> it = items[0];
       const float c = a.scale * 1.4426950408889634f;
       const uint32_t part = smem_u32(smem), ml = part + C::kShareO;
