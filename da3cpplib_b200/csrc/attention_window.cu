@@ -950,6 +950,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * 2 * C::kTile);
   uint64_t* empty = full + C::kStages;
+  uint32_t* gave_up = reinterpret_cast<uint32_t*>(empty + C::kStages);  // not 0: a wait of this CTA ran out
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = static_cast<int>(blockIdx.x) % nsplit, item = static_cast<int>(blockIdx.x) / nsplit;
@@ -1117,7 +1118,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 
   // Join the warps: each leaves O, maxima and sums in the ring (every tile has been read).
   // part[w]: [16][D], then [16] maxima, [16] sums; part[kFewWarps] is the CTA's.
-  const int bad = __syncthreads_or(!ok);
+  uint32_t bad = __syncthreads_or(!ok);
+  if (threadIdx.x == 0) *gave_up = bad;
   float* part = reinterpret_cast<float*>(smem);
   if (warp < kFewWarps) {
     float* w = part + warp * C::kPartFloats;
@@ -1166,8 +1168,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
   if (nsplit > 1) cluster_sync();
   else __syncthreads();
-  // Join the CTAs of the cluster in rank order; each writes its share of the elements.
-  if (!bad) {
+  // Join the CTAs of the cluster in rank order; each writes its share of the elements, unless a
+  // wait of any of them ran out.
+  if (nsplit > 1)
+    for (int i = 0; i < nsplit; ++i) bad |= __float_as_uint(ld_dsmem_f1(mapa_shared(smem_u32(gave_up), i)));
+  if (bad == 0) {
     const uint32_t base = smem_u32(mine);
     const int pairs = rows * D / 2;
     for (int e = split * kFewThreads + static_cast<int>(threadIdx.x); e < pairs; e += nsplit * kFewThreads) {

@@ -47,3 +47,8 @@ def whole_rows_or_none(lib, B, Tq, Tk, h, kvh, D, left, right, sinks):
 ])
 def test_split_items(lib, B, Tq, Tk, h, kvh, D, left, right, sinks):
     whole_rows_or_none(lib, B, Tq, Tk, h, kvh, D, left, right, sinks)
+
+
+@pytest.mark.parametrize("B,Tq,Tk,h,kvh,D", [(1, 1, 20000, 4, 4, 64), (2, 2, 20000, 8, 2, 128)])
+def test_few_queries(lib, B, Tq, Tk, h, kvh, D):
+    whole_rows_or_none(lib, B, Tq, Tk, h, kvh, D, -1, 0, 3)
