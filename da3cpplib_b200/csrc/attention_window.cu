@@ -100,13 +100,14 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // 2^x of two values on the FMA pipe (the MUFU pipe takes one exponential a score
-// otherwise, and bounds the kernel): x = j + f with j = round(x) (adding 1.5 * 2^23 leaves j
-// in the low mantissa bits), f in [-0.5, 0.5]; 2^f by a cubic fitted to relative error
-// (max 7.5e-5, below the rounding of P to 16 bits); j is added to the exponent field. x is
-// held at -125, where the result rounds to 0 in f16 and to 2^-125 in bf16 (at most 2^-117 of
-// the row's largest probability).
+// otherwise, and bounds the kernel): x = j + f with j = round(x) (adding 1.5 * 2^23 + 127
+// leaves j + 127 in the low mantissa bits), f in [-0.5, 0.5]; 2^f by a cubic fitted to
+// relative error (max 7.5e-5, below the rounding of P to 16 bits), times 2^j, whose bits are
+// j + 127 in the exponent field. (Adding j to the cubic's own exponent field would turn NaN
+// into a number.) x is held at -125, where the result rounds to 0 in f16 and to 2^-125 in bf16
+// (at most 2^-117 of the row's largest probability).
 __device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  constexpr float kShift = 12582912.0f;
+  constexpr float kShift = 12582912.0f + 127.0f;
   constexpr float c3 = 0.05517166853f, c2 = 0.24261112511f, c1 = 0.69326096773f, c0 = 0.99992805719f;
   x = make_float2(fmax_nan(x.x, -125.0f), fmax_nan(x.y, -125.0f));
   const float2 t = __fadd2_rn(x, make_float2(kShift, kShift));
@@ -115,8 +116,8 @@ __device__ __forceinline__ float2 exp2_cubic(float2 x) {
   float2 p = __ffma2_rn(make_float2(c3, c3), f, make_float2(c2, c2));
   p = __ffma2_rn(p, f, make_float2(c1, c1));
   p = __ffma2_rn(p, f, make_float2(c0, c0));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  return __fmul2_rn(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23),
+                                   __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 
 // N columns (a multiple of 16) of this thread's lane of tensor memory, there after
