@@ -104,12 +104,12 @@ __device__ __forceinline__ float ex2(float x) {
 // leaves j + 127 in the low mantissa bits), f in [-0.5, 0.5]; 2^f by a cubic fitted to
 // relative error (max 7.5e-5, below the rounding of P to 16 bits), times 2^j, whose bits are
 // j + 127 in the exponent field. (Adding j to the cubic's own exponent field would turn NaN
-// into a number.) x is held at -125, where the result rounds to 0 in f16 and to 2^-125 in bf16
-// (at most 2^-117 of the row's largest probability).
+// into a number.) x is held at -127, where those bits and so the result are zero: a masked score
+// has no weight at all, whatever value it would meet in V.
 __device__ __forceinline__ float2 exp2_cubic(float2 x) {
   constexpr float kShift = 12582912.0f + 127.0f;
   constexpr float c3 = 0.05517166853f, c2 = 0.24261112511f, c1 = 0.69326096773f, c0 = 0.99992805719f;
-  x = make_float2(fmax_nan(x.x, -125.0f), fmax_nan(x.y, -125.0f));
+  x = make_float2(fmax_nan(x.x, -127.0f), fmax_nan(x.y, -127.0f));
   const float2 t = __fadd2_rn(x, make_float2(kShift, kShift));
   const float2 j = __fadd2_rn(t, make_float2(-kShift, -kShift));
   const float2 f = __fadd2_rn(x, make_float2(-j.x, -j.y));
@@ -678,8 +678,8 @@ __global__ void __launch_bounds__(WinCfg<D>::kThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok);
       if (nsplit == 1) {
-        // O / l. A row that saw no key still has m = -inf and is zero (exp2_cubic gives its
-        // masked scores 2^-125, not 0); one of NaN scores has m = -inf too, but l is NaN.
+        // O / l. A row that saw no key still has m = -inf and is zero; one of NaN scores has
+        // m = -inf too, but l is NaN.
         const float inv = m == -INFINITY && l == l ? 0.f : 1.f / l;
         const Item<KT> it = items[k & 1];
         const bool mine = ok && r < it.span(a, tokens, t).n * g;
