@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -1314,7 +1315,9 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
   a.left = left < 0 || left > kWindowAll ? kWindowAll : left;
   a.right = right < 0 || right > kWindowAll ? kWindowAll : right;
   a.sinks = sinks;
-  a.scale = fmaxf(scale, 1e-30f);  // at 0 a masked score (-inf) times it would be NaN
+  // At 0 a masked score (-inf) times it would be NaN. Times the smallest float any f32 score is
+  // below 2^-20, and every weight 1.
+  a.scale = fmaxf(scale, FLT_TRUE_MIN);
   if (!take_strides(q_strides, nseq, q_len, heads, head_dim, &a.qs) ||
       (k_len > 0 && (!take_strides(k_strides, nseq, k_len, kv_heads, head_dim, &a.ks) ||
                      !take_strides(v_strides, nseq, k_len, kv_heads, head_dim, &a.vs))) ||
