@@ -22,16 +22,18 @@ namespace da3b {
 namespace {
 
 // 16 consecutive values x[c .. c + 15] of a row as f32, zeros from column K on. VEC: K is
-// a multiple of 16 and the row starts on a 32-byte boundary.
+// a multiple of 16 and the row starts on a 32-byte boundary. Plain loads, not those of the
+// read-only path (nor of pointers that the compiler may take for it): a kernel that starts
+// while the one ahead of it is still running may be reading what that one writes.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load16(const T* __restrict__ row, int c, int K, float (&v)[16]) {
+__device__ __forceinline__ void load16(const T* row, int c, int K, float (&v)[16]) {
   if (VEC) {
     if (c < K) {
       // 32 bytes a load: a warp's loads cover 1024 consecutive bytes
       uint32_t w[sizeof(T) * 4];
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-        asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(w[8 * i]), "=r"(w[8 * i + 1]), "=r"(w[8 * i + 2]), "=r"(w[8 * i + 3]), "=r"(w[8 * i + 4]),
                        "=r"(w[8 * i + 5]), "=r"(w[8 * i + 6]), "=r"(w[8 * i + 7])
                      : "l"(reinterpret_cast<const uint32_t*>(row + c) + 8 * i));
@@ -102,7 +104,7 @@ __device__ __forceinline__ void store_fp8(float (&v)[16], int r, int c0, int K, 
 // warps wait for their loads, with 4 KB in flight each and 31 of them an SM.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-    k_quantize_fp8(const T* __restrict__ x, int rows, int K, int ldx, uint8_t* __restrict__ q, int ldq,
+    k_quantize_fp8(const T* x, int rows, int K, int ldx, uint8_t* __restrict__ q, int ldq,
                    uint8_t* __restrict__ scales) {
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);
   pdl_trigger();
@@ -124,8 +126,8 @@ __global__ void __launch_bounds__(256)
 // columns; rows of at most 2048 columns take one warp, longer ones eight.
 template <int WARPS, int NV, bool VEC>
 __global__ void __launch_bounds__(256)
-    k_layernorm_fp8(const float* __restrict__ x, int rows, int K, int ldx, const float* __restrict__ g,
-                    const float* __restrict__ b, float eps, uint8_t* __restrict__ q, int ldq,
+    k_layernorm_fp8(const float* x, int rows, int K, int ldx, const float* g,
+                    const float* b, float eps, uint8_t* __restrict__ q, int ldq,
                     uint8_t* __restrict__ scales) {
   __shared__ float part[2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(256)
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        y[i] = c + i < K ? (v[j][i] - mean) * rstd * __ldg(g + c + i) + (b ? __ldg(b + c + i) : 0.f) : 0.f;
+        y[i] = c + i < K ? (v[j][i] - mean) * rstd * g[c + i] + (b ? b[c + i] : 0.f) : 0.f;
     }
     store_fp8(y, r, c0, K, q, ldq, scales + fp8_scale_offset(r, c0 >> 7, row_tiles));
   }
@@ -196,8 +198,8 @@ constexpr int kWalkBlocks = NV == 1 ? 5 : 3;  // resident on an SM, by registers
 
 template <int NV>
 __global__ void __launch_bounds__(128, kWalkBlocks<NV>)
-    k_layernorm_fp8_walk(const float* __restrict__ x, int rows, int K, int ldx, const float* __restrict__ g,
-                         const float* __restrict__ b, float eps, uint8_t* __restrict__ q, int ldq,
+    k_layernorm_fp8_walk(const float* x, int rows, int K, int ldx, const float* g,
+                         const float* b, float eps, uint8_t* __restrict__ q, int ldq,
                          uint8_t* __restrict__ scales) {
   const int lane = threadIdx.x & 31, step = gridDim.x * 4;
   const int row_tiles = (rows + 127) / 128;

@@ -485,8 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int n = n0 + lane + 32 * i;
-        ctab[lane + 32 * i] = a.bias && n < a.N ? __ldg(a.bias + n) : 0.f;
-        ctab[64 + lane + 32 * i] = a.scale && n < a.N ? __ldg(a.scale + n) : 1.f;
+        ctab[lane + 32 * i] = a.bias && n < a.N ? a.bias[n] : 0.f;
+        ctab[64 + lane + 32 * i] = a.scale && n < a.N ? a.scale[n] : 1.f;
       }
       __syncwarp();
       if (!mbar_wait_warp(&tfull[acc], (it / C::kAcc) & 1, status, kStatusTimeoutAccum)) break;
