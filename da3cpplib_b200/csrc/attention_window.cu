@@ -1236,6 +1236,7 @@ int launch_few(const AttnWindow& a, int* status, cudaStream_t s) {
 
 // No keys at all (k_len 0; a tensor map cannot be empty): zeros in the rows that count.
 __global__ void k_attn_none(const AttnWindow a) {
+  pdl_wait();
   const int64_t per_row = a.head_dim / 8;
   const int64_t n = static_cast<int64_t>(a.nseq) * a.q_len * a.heads * per_row;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < n;
@@ -1260,10 +1261,7 @@ static int run(const AttnWindow& a, int* status, cudaStream_t s) {
 }
 
 int attention_window(const AttnWindow& a, int* status, cudaStream_t s) {
-  if (a.k_len == 0) {
-    k_attn_none<<<256, 256, 0, s>>>(a);
-    return cudaGetLastError() == cudaSuccess ? 0 : -4;
-  }
+  if (a.k_len == 0) return launch_pdl(k_attn_none, dim3(256), 256, 0, s, 1, a) == cudaSuccess ? 0 : -4;
   if (a.bf16) return a.head_dim == 64 ? run<64, true>(a, status, s) : run<128, true>(a, status, s);
   return a.head_dim == 64 ? run<64, false>(a, status, s) : run<128, false>(a, status, s);
 }

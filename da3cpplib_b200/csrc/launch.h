@@ -10,7 +10,8 @@
 
 namespace da3b {
 
-// cluster: CTAs a cluster along x (1: none).
+// cluster: CTAs a cluster along x (1: none). A launch that fails leaves no error behind for
+// cudaGetLastError, which the next call would take for its own.
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
                        unsigned cluster, const Args&... args) {
@@ -27,7 +28,9 @@ cudaError_t launch_pdl(void (*kernel)(Params...), dim3 grid, unsigned threads, s
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
 }
 
 // Whether kernels can use these buffers: memory of the current device, or managed or pinned
