@@ -1323,6 +1323,8 @@ DA3B_API int da3b_attention_window(const void* q, const int64_t* q_strides, cons
     return -1;
   for (const void* p : {q, k, v, static_cast<const void*>(out)})
     if (reinterpret_cast<uintptr_t>(p) & 15) return -1;
+  for (const int* p : {q_lens, k_lens})
+    if (reinterpret_cast<uintptr_t>(p) & 3) return -1;
   // 32-bit work counts inside
   if (static_cast<double>(nseq) * heads * q_len > 2147483647.0 * 8) return -1;
   if (!usable_here({q, k_len > 0 ? k : nullptr, k_len > 0 ? v : nullptr, out, q_lens, k_lens})) return -104;
