@@ -306,8 +306,11 @@ bool usable_here(std::initializer_list<const void*> buffers) {
     int at = -1;
     if (ask(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, d) != CUDA_SUCCESS) return false;
     if (at == dev) continue;
-    unsigned type = 0;  // pinned memory belongs to no device in particular
-    if (ask(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, d) != CUDA_SUCCESS || type != CU_MEMORYTYPE_HOST) return false;
+    // pinned and managed memory belong to no device in particular (the one named is that which
+    // was current when they were allocated)
+    unsigned type = 0, managed = 0;
+    if (ask(&type, CU_POINTER_ATTRIBUTE_MEMORY_TYPE, d) == CUDA_SUCCESS && type == CU_MEMORYTYPE_HOST) continue;
+    if (ask(&managed, CU_POINTER_ATTRIBUTE_IS_MANAGED, d) != CUDA_SUCCESS || !managed) return false;
   }
   return true;
 }
