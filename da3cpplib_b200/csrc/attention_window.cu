@@ -299,7 +299,7 @@ struct Seen {
 
 // The keys of a CTA as one run of columns: the sinks, up to a multiple of eight, then the
 // windows' keys from the oldest on, so that neither starts a tile of its own: four sinks and
-// a window of 1024 for 64 tokens are 9 tiles of 128 instead of 11. One tile may hold both; it
+// a window of 1024 for 64 tokens are 18 tiles of 64 instead of 19. One tile may hold both; it
 // is loaded in boxes of eight rows.
 struct Columns {
   int front;  // columns of the sinks (0: the columns are keys from `base` on)
@@ -1226,7 +1226,8 @@ int launch_few(const AttnWindow& a, int* status, cudaStream_t s) {
   const int64_t items = static_cast<int64_t>(a.nseq) * a.kv_heads;
   const int64_t window = static_cast<int64_t>(a.left) + a.q_len + a.sinks;
   const int64_t tiles = (std::min<int64_t>(a.k_len, window) + kFewKeys - 1) / kFewKeys;
-  const int nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 296 / items, tiles / 4})));
+  const int64_t slots = 2 * static_cast<int64_t>(sm_count(dev));
+  const int nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, slots / items, tiles / 4})));
   if (items * nsplit > 0x7fffffff) return -1;
   return launch_pdl(k_attn_few<D, BF16>, dim3(static_cast<unsigned>(items * nsplit)), kFewThreads, C::kSmem, s,
                     static_cast<unsigned>(nsplit), tk, tv, a, nsplit, status) == cudaSuccess
@@ -1254,8 +1255,10 @@ __global__ void k_attn_none(const AttnWindow a) {
 
 template <int D, bool BF16>
 static int run(const AttnWindow& a, int* status, cudaStream_t s) {
-  // few rows for each key head: the memory-bound kernel (its tensor work is padded to 16
-  // rows, the tiled kernel's to 256)
+  // few rows for each key head: the memory-bound kernel (its tensor work is padded to 16 rows,
+  // the tiled kernel's to 128 a query tile). 32 single tokens, 8 key heads of 128 dims, windows
+  // of 4096: 16 rows a key head here 87 us, 17 rows there 120; 16 key heads of 64 dims over 6485
+  // keys: 16 queries here 14 us, 17 there 21.
   if (static_cast<int64_t>(a.q_len) * (a.heads / a.kv_heads) <= kFewRows) return launch_few<D, BF16>(a, status, s);
   return launch_tiles<D, BF16>(a, status, s);
 }

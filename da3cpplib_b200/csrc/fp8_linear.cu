@@ -20,16 +20,16 @@
 //              buffer, stored (or, onto the residual, added) by TMA: the load-store unit,
 //              73 % busy with the pieces' reads and stores when the warps made them, only
 //              writes the buffer. Four warps an SM sub-partition hide each other's
-//              latencies: M = 87680, K = 1024, N = 4096 with GELU to f16 takes 410-460 us,
-//              eight warps of 128 columns took 528-580.
+//              latencies: eight warps of 128 columns took a quarter longer (M = 87680,
+//              K = 1024, N = 4096 with GELU to f16).
 //
 // Bound: long reductions by the chip's power (8192 x 8192 x 8192: 440 us or 2.5 PFLOP/s, the
 // MMAs at 92 % of their cycles but at 1.1 GHz), short ones by the MMAs (K = 1024: 4096 cycles a
 // 256 x 256 tile) and the handover of a pair's one accumulator to the epilogue and back, about
 // 1600 cycles: M = 87680, N = 4096 takes 315 us (2.3 PFLOP/s), M = 21920 85; K = 4096, N = 1024
 // 74. With GELU the epilogue's own instructions (17 a value, two of them MUFU) are as long as
-// the MMAs: 100 us at M = 21920, 96 quantised. A ring of five stages: four and six measured
-// the same.
+// the MMAs: 101 us at M = 21920, 104 quantised, 376 at M = 87680. A ring of five stages: four
+// and six measured the same.
 // Every wait is bounded (ptx.cuh); on a timeout the kernel records a status and exits.
 #include <algorithm>
 #include <atomic>
@@ -131,8 +131,8 @@ __device__ __forceinline__ void copy_sf(uint32_t tmem, uint32_t saddr) {
 // 6.8e-8; beyond 6, v^2 is held at 36 and Phi is 0 or 1 to 1e-9. Ten multiply-adds and two
 // MUFU operations a value; the four pairs run side by side, because a chain of about
 // fifteen dependent operations a value otherwise leaves the pipes idle (the M = 87680,
-// K = 1024, N = 4096 product with GELU: 723 us with one chain at a time, 400-430 so). One
-// reciprocal for two values (of the product of their denominators) was no faster: 417-430.
+// K = 1024, N = 4096 product with GELU took 1.7 times as long with one chain at a time). One
+// reciprocal for two values (of the product of their denominators) was no faster.
 __device__ __forceinline__ void gelu8(float* v) {
   float2 x[4], q[4];
   const float2 one = make_float2(1.f, 1.f);
@@ -597,9 +597,9 @@ int check_linear_fp8(const Fp8Linear& a) {
 int linear_fp8(const Fp8Linear& a, int* status, cudaStream_t s) {
   // The tile shape with the shorter time (ns): waves of tiles times a tile's k-blocks of 128,
   // and the handover from one tile to the next, longer with a pair's one accumulator; pairs
-  // also take longer to set up. Measured at N = 4096, K = 1024 and M = 512, 1370, 2740, 5480,
-  // 21920: single CTAs 6.5, 11.3, 16.2, 28, 105 us, pairs 8.9, 12.3, 15.8, 23, 85; at N = 1024,
-  // K = 4096 and M = 1370, 2740: 13.6 and 22.8, 17.7 and 18.4.
+  // also take longer to set up. Measured back to back in a graph, at N = 4096, K = 1024 and M =
+  // 512, 1370, 2740, 5480, 21920: single CTAs 7.0, 12.0, 17.7, 30, 107 us, pairs 8.8, 12.3, 16.2,
+  // 23, 87; at N = 1024, K = 4096 and M = 1370, 2740: 15.2 and 25, 17.7 and 17.3.
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t sms = sm_count(dev), kb = (a.K + 127) / 128;
