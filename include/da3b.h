@@ -185,12 +185,14 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  *
  * A matrix [rows][K] (activations, or weights [N][K]) is held as e4m3 codes [rows][ld]
  * (ld bytes, ld >= K and a multiple of 16, base 16-byte aligned) and one scale for each
- * row and 128 columns: value = code * 2^(s - 127), s a byte of at most 254. The scale bytes lie in
- * "scale tiles" (16-byte aligned, da3b_fp8_scale_bytes(rows, K) bytes): 512 bytes for each
- * 512 columns g and 128 rows t, in the order [g][t][32][4][4]; row 128 t + 32 c + l and
+ * row and 128 columns: value = code * 2^(s - 127), s a byte of at most 254. The scale bytes
+ * lie in "scale tiles" (16-byte aligned, da3b_fp8_scale_bytes(rows, K) bytes): 512 bytes for
+ * each 512 columns g and 128 rows t, in the order [g][t][32][4][4]; row 128 t + 32 c + l and
  * columns from 128 (4 g + j) on have theirs at [g][t][l][c][j]. Bytes of rows and columns
  * that the matrix does not have are never used. The tiles depend on the number of rows:
- * pass the same `rows` everywhere.
+ * pass the same `rows` everywhere. This is the only form that the linears take: weights with
+ * power-of-two scales for blocks of 128 x 128 have each scale repeated for the block's rows;
+ * weights with scales that are no powers of two have to be quantised anew.
  *
  * A quantised block has the smallest s with max|x| <= 448 * 2^(s - 127) (at least 0; 127
  * for a block of zeros), codes round to nearest, ties to even. e4m3 has no infinity:
@@ -198,7 +200,8 @@ DA3B_API int da3b_attention_noalloc(const void* qkv, int nseq, int seqlen, int h
  *
  * Types: 0 f16, 1 bf16, 2 f32. All functions return 0 when launched, -100 for a null
  * pointer (one to a buffer without rows may be null) or a bad code or count, -1 for sizes,
- * leading dimensions or alignments that are not served, -104 for a buffer that is not memory of the current device (or pinned or
+ * leading dimensions or alignments that are not served (and a dtype that the quantiser does
+ * not know), -104 for a buffer that is not memory of the current device (or pinned or
  * managed), other negative values for launch errors. Calls with no rows do nothing.
  * Nothing is allocated except the status word on a device's first call; any number of
  * calls may run at once, and a stream may capture any of them. Pointers belong to the
@@ -213,12 +216,14 @@ DA3B_API int da3b_quantize_fp8(const void* x, int dtype, int rows, int K, int ld
 
 /* LayerNorm of f32 rows, (x - mean) / sqrt(var + eps) * gamma + beta (beta may be NULL;
  * K <= 16384), quantised as above: the norm before a block's linears, without the f16
- * round trip. */
+ * round trip. Mean and variance are f32 sums over the row, one after the other: a value next
+ * to a border of e4m3 may fall the other way than in exact arithmetic. */
 DA3B_API int da3b_layernorm_fp8(const float* x, int rows, int K, int ldx, const float* gamma, const float* beta,
                                 float eps, void* q, int ldq, void* scales, void* stream);
 
 /* y = act(x w^T + bias) of quantised x [M][K] and w [N][K]; bias f32 [N] or NULL, act as
- * da3b_linear_f16 (2 and 3 are the same erf-form GELU here), sums in f32.
+ * da3b_linear_f16, sums in f32. 2 and 3 are the same GELU here, a logistic form fitted to the
+ * erf form within 7e-8 and evaluated in f32, whatever the type of the output.
  *   da3b_linear_fp8:           y [M][ldo] of type out_dtype.
  *   da3b_linear_fp8_q:         y quantised by the product's epilogue: codes out_q [M][ldo]
  *                              (ldo a multiple of 16, columns from N on untouched) and
@@ -247,7 +252,9 @@ DA3B_API int da3b_linear_fp8_resid_f32(const void* x, int M, int K, int ldx, con
  * left, right < 0: no limit on that side. right = 0 is causal; one query per sequence is
  * the form for single tokens over a cache. out = sum_j softmax_j(scale * q.k_j) v_j with
  * f32 statistics; a query that sees no key gets zeros, rows from ql on are left as they
- * were. Keys that no query of the sequence sees are never used, whatever they hold (NaN
+ * were. The weights are rounded to the inputs' type before they meet v (f16 keeps less than
+ * its 11 bits of those below 2^-14 of a reference within 2^8 of the row's largest), the sum
+ * that divides is of the unrounded ones, and a quarter of the exponentials are good to 7.5e-5. Keys that no query of the sequence sees are never used, whatever they hold (NaN
  * and infinities included); a key that some query sees has to be finite for all of them.
  *
  * q, out [nseq][q_len][heads][head_dim], k, v [nseq][k_len][kv_heads][head_dim], each with
